@@ -472,6 +472,72 @@ int lat_row_norm(
     int32_t dtype, int32_t rms, const void* feats, int64_t rows, int32_t channels,
     const void* weight, const void* bias, float eps, void* out, void* stream);
 
+/* The same normalisation for training (no counterpart in the reference's native extension:
+ * its array library differentiates layer_norm / rms_norm). Rows of `feats` are
+ * feat_row_stride elements apart, `out` is dense. Leaves the row statistics in float32: mean
+ * [rows] (layer norm only, else NULL) and rstd [rows] = 1 / sqrt(variance + eps). */
+int lat_row_norm_forward(
+    int32_t dtype, int32_t rms, const void* feats, int64_t rows, int32_t channels, int64_t feat_row_stride,
+    const void* weight, const void* bias, float eps, void* out, float* mean, float* rstd, void* stream);
+
+/* Gradients of lat_row_norm_forward: grad_feats [rows, channels], and grad_weight / grad_bias
+ * [channels] unless NULL (with both NULL no workspace is needed). With xh = (x - mean) rstd and
+ * g = grad * weight: grad_feats = rstd (g - mean(g) - xh mean(g xh)), without mean(g) for RMS;
+ * grad_weight = sum over rows of grad * xh; grad_bias = sum over rows of grad. Sums in float32,
+ * in a fixed order; each result is cast once. */
+size_t lat_row_norm_backward_workspace_bytes(int64_t rows, int32_t channels);
+int lat_row_norm_backward(
+    int32_t dtype, int32_t rms, const void* grad, int64_t grad_row_stride, const void* feats, int64_t rows,
+    int32_t channels, int64_t feat_row_stride, const void* weight, const float* mean, const float* rstd,
+    void* grad_feats, void* grad_weight, void* grad_bias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* mlx_lattice/ops/feature.py:132-150 (`dropout` in training mode), with a mask that is a
+ * function of a counter: element i stays where word i % 4 of Philox4x32-10 (counter: i / 4 in
+ * the two low words, `offset` in the two high words; key: seed) is at least round(p 2^32), and
+ * is then scaled by 1 / (1 - p); other elements give 0 whatever they hold. `residual` (or NULL)
+ * is added afterwards, before the one cast. seed_device (or NULL): a device word that takes the
+ * place of `seed`, read when the kernel runs, so that a replayed graph can draw new masks. The
+ * gradient is the same call on the gradient of the output, without a residual. */
+int lat_dropout(
+    int32_t dtype, const void* feats, const void* residual, int64_t elements, double p, uint64_t seed,
+    const uint64_t* seed_device, uint64_t offset, void* out, void* stream);
+
+/* Gated linear recurrence over the rows of each sequence (no counterpart in the reference):
+ * a_t = sigmoid(gate_t), h_t = a_t h_{t-1} + (1 - a_t) x_t per channel; the h before the first
+ * row is initial_state [sequences, channels] float32 (NULL: zero). Sequence j holds the rows
+ * offsets[j] .. offsets[j + 1] - 1 (device int32, sequences + 1 entries, rising; entries are
+ * clamped to 0 .. rows, falling ones raise LAT_STATUS_BAD_INDEX); `reverse` runs every sequence
+ * from its last row to its first. Rows outside all sequences give zeros. out [rows, channels]
+ * is dense; final_state [sequences, channels] float32 (or NULL) is the h after the last row (an
+ * empty sequence hands its initial state on). carries (NULL unless a backward pass follows):
+ * float32 [lat_recurrence_tiles(rows), channels]. One pass; bitwise repeatable. A wait on
+ * another block that runs out of its budget raises LAT_STATUS_WAIT_TIMEOUT. */
+size_t lat_recurrence_workspace_bytes(int32_t rows, int32_t channels);
+int32_t lat_recurrence_tiles(int32_t rows);
+int lat_recurrence_forward(
+    int32_t dtype, const void* feats, int64_t feat_row_stride, const void* gate, int64_t gate_row_stride,
+    int32_t rows, int32_t channels, const int32_t* offsets, int32_t sequences, const float* initial_state,
+    int32_t reverse, void* out, float* final_state, float* carries, void* workspace, size_t workspace_bytes,
+    int32_t* status, void* stream);
+
+/* Gradients of lat_recurrence_forward from grad [rows, channels] and grad_final [sequences,
+ * channels] float32 (or NULL): grad_feats and grad_gate [rows, channels] dense, zero outside
+ * all sequences; grad_initial [sequences, channels] float32 or NULL. `carries` as the forward
+ * call left it; h is computed again from it in float32. */
+int lat_recurrence_backward(
+    int32_t dtype, const void* grad, int64_t grad_row_stride, const float* grad_final, const void* feats,
+    int64_t feat_row_stride, const void* gate, int64_t gate_row_stride, int32_t rows, int32_t channels,
+    const int32_t* offsets, int32_t sequences, const float* initial_state, int32_t reverse, const float* carries,
+    void* grad_feats, void* grad_gate, float* grad_initial, void* workspace, size_t workspace_bytes,
+    int32_t* status, void* stream);
+
+/* One row of every stream: next_state = a state + (1 - a) x with a = sigmoid(gate), `out` the
+ * same rounded to the feature type. state and next_state [rows, channels] float32; next_state
+ * may be state itself. */
+int lat_recurrence_step(
+    int32_t dtype, const void* feats, int64_t feat_row_stride, const void* gate, int64_t gate_row_stride,
+    const float* state, int64_t rows, int32_t channels, void* out, float* next_state, void* stream);
+
 /* mlx_lattice/ops/feature.py:59-129: op 0 sigmoid, 1 silu, 2 tanh, 3 gelu (erf form),
  * 4 gelu (tanh approximation), 5 gelu (x * sigmoid(1.702 x)), 6 leaky_relu (p0 = negative
  * slope), 7 softplus (p0 = beta > 0, p1 = threshold: x where beta x > threshold, else

@@ -8,7 +8,9 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import (
+    POINTER, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_uint64, c_void_p,
+)
 
 _PACKAGE_DIR = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(_PACKAGE_DIR, 'liblattice_b200.so')
@@ -108,6 +110,18 @@ SIGNATURES = {
     'lat_relu': (I, [I, P, c_int64, P, P]),
     'lat_activation': (I, [I, I, P, c_int64, c_float, c_float, P, P]),
     'lat_row_norm': (I, [I, I, P, c_int64, I, P, P, c_float, P, P]),
+    'lat_row_norm_forward': (I, [I, I, P, c_int64, I, c_int64, P, P, c_float, P, P, P, P]),
+    'lat_row_norm_backward_workspace_bytes': (c_size_t, [c_int64, I]),
+    'lat_row_norm_backward': (
+        I, [I, I, P, c_int64, P, c_int64, I, c_int64, P, P, P, P, P, P, P, c_size_t, P]),
+    'lat_dropout': (I, [I, P, P, c_int64, c_double, c_uint64, P, c_uint64, P, P]),
+    'lat_recurrence_workspace_bytes': (c_size_t, [I, I]),
+    'lat_recurrence_tiles': (I, [I]),
+    'lat_recurrence_forward': (
+        I, [I, P, c_int64, P, c_int64, I, I, P, I, P, I, P, P, P, P, c_size_t, P, P]),
+    'lat_recurrence_backward': (
+        I, [I, P, c_int64, P, P, c_int64, P, c_int64, I, I, P, I, P, I, P, P, P, P, P, c_size_t, P, P]),
+    'lat_recurrence_step': (I, [I, P, c_int64, P, c_int64, P, c_int64, I, P, P, P]),
     'lat_concat_aligned_features': (I, [I, P, P, I, I, P, P, I, I, c_int64, P, P, P]),
     'lat_binary_aligned_features': (
         I, [I, I, P, P, I, c_float, P, P, I, c_float, c_int64, I, P, P, P]),

@@ -26,12 +26,13 @@ SOURCES = (
     'static_scratch.cu',
     'pool.cu',
     'feature.cu', 'align.cu',
+    'row_norm.cu', 'dropout.cu', 'recurrence.cu',
     'capi.cu',
 )
 
 NVCC_FLAGS = (
     '-gencode', 'arch=compute_100a,code=sm_100a',
-    '-lineinfo', '-O3', '-std=c++17',
+    '-lineinfo', '-O3', '-std=c++17', '-t', '0',
     '-Xcompiler', '-fPIC', '-shared',
 )
 

@@ -29,9 +29,10 @@ from mlx_lattice_b200.nn.quantized_conv import (
     QuantizedSubmConv3d,
 )
 from mlx_lattice_b200.nn.quantized_feature import QuantizedLinear
+from mlx_lattice_b200.nn.recurrence import GatedRecurrence
 
 __all__ = [
-    'Dropout', 'GELU', 'LayerNorm', 'LeakyReLU', 'RMSNorm', 'SiLU', 'Sigmoid', 'Softplus', 'Tanh',
+    'Dropout', 'GELU', 'GatedRecurrence', 'LayerNorm', 'LeakyReLU', 'RMSNorm', 'SiLU', 'Sigmoid', 'Softplus', 'Tanh',
     'AvgPool3d', 'BatchNorm', 'Conv3d', 'ConvTranspose3d', 'GlobalAvgPool', 'GlobalMaxPool',
     'GlobalSumPool', 'Linear', 'MaxPool3d', 'Module', 'Pool3d', 'QuantizedConv3d',
     'QuantizedConvTranspose3d', 'QuantizedLinear', 'QuantizedSubmConv3d', 'ReLU', 'SubmConv3d',

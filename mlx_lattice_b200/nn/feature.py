@@ -91,15 +91,16 @@ class Softplus(Module):
 
 
 class Dropout(Module):
-    """Inference module: features pass unchanged (``nn/feature.py:134-145``, evaluation)."""
+    """``nn/feature.py:134-145``. Without a ``seed`` the features pass unchanged (evaluation);
+    with one the call drops elements. ``residual`` is added in the same pass."""
 
     def __init__(self, p: float = 0.5) -> None:
         if p < 0 or p >= 1:
             raise ValueError('p must satisfy 0 <= p < 1.')
         self.p = p
 
-    def __call__(self, x: SparseTensor) -> SparseTensor:
-        return F.dropout(x, p=self.p, training=False)
+    def __call__(self, x: SparseTensor, *, seed=None, offset: int = 0, residual=None) -> SparseTensor:
+        return F.dropout(x, p=self.p, training=seed is not None, seed=seed, offset=offset, residual=residual)
 
 
 class LayerNorm(Module):

@@ -44,6 +44,11 @@ from mlx_lattice_b200.ops.quantization import (
     voxelize,
     voxelize_with_quantization,
 )
+from mlx_lattice_b200.ops.recurrence import (
+    gated_recurrence,
+    gated_recurrence_step,
+    sequence_offsets,
+)
 from mlx_lattice_b200.ops.tensor import (
     align_sparse,
     sparse_add,
@@ -60,6 +65,7 @@ __all__ = [
     'dropout', 'gelu', 'layer_norm', 'leaky_relu', 'rms_norm', 'sigmoid', 'silu', 'softplus', 'tanh',
     'align_sparse', 'sparse_add', 'sparse_binary_op', 'sparse_maximum', 'sparse_minimum', 'sparse_mul',
     'sparse_sub',
+    'gated_recurrence', 'gated_recurrence_step', 'sequence_offsets',
     'avg_pool3d', 'batch_norm', 'build_generative_relation', 'build_point_voxel_map', 'devoxelize',
     'interpolate_point_features', 'build_kernel_relation',
     'build_submanifold_kernel_relation', 'build_target_kernel_relation',

@@ -6,6 +6,7 @@ import torch
 
 from mlx_lattice_b200 import _ext
 from mlx_lattice_b200.core import QuantizedWeight, SparseTensor
+from mlx_lattice_b200.ops import _autograd
 from mlx_lattice_b200.ops._quantized import quantized_matmul
 
 __all__ = [
@@ -69,28 +70,56 @@ def softplus(x: SparseTensor, *, beta: float = 1.0, threshold: float = 20.0) -> 
     return x.replace(feats=_ext.activation(x.feats, 'softplus', float(beta), float(threshold)))
 
 
-def dropout(x: SparseTensor, *, p: float = 0.5, training: bool = True) -> SparseTensor:
-    """Inference form of ``ops/feature.py:132-150``: the features pass unchanged when
-    ``training`` is false or ``p`` is zero. Sampling a mask is training work and is not
-    part of this package."""
+def dropout(
+    x: SparseTensor, *, p: float = 0.5, training: bool = True, seed=None, offset: int = 0,
+    residual=None,
+) -> SparseTensor:
+    """Dropout of ``ops/feature.py:132-150``: each element stays with probability ``1 - p`` and
+    is then scaled by ``1 / (1 - p)``. The features pass unchanged when ``training`` is false or
+    ``p`` is zero.
+
+    The mask is a function of ``seed``, ``offset`` and the element's place in the feature array;
+    it is never stored, and the gradient draws it again. ``seed`` (required in training mode) is
+    an int, or an int64 CUDA tensor of one element that is read when the kernel runs: change it
+    between the replays of a captured graph to draw new masks. ``offset`` separates the layers
+    that share a seed. ``residual`` (a tensor like ``x.feats``, or a ``SparseTensor`` over the
+    same coordinates) is added in the same pass."""
     if p < 0 or p >= 1:
         raise ValueError('p must satisfy 0 <= p < 1.')
-    if training and p != 0:
-        raise ValueError('dropout in training mode is not available on the inference path.')
-    return x.replace(feats=x.feats)
+    if training and p != 0 and seed is None:
+        raise ValueError('dropout in training mode needs a seed.')
+    if isinstance(residual, SparseTensor):
+        if not residual.same_coords(x):
+            raise ValueError('residual must share the coordinates of x.')
+        residual = residual.feats
+    if not training or p == 0:
+        if residual is None:
+            return x.replace(feats=x.feats)
+        p, seed = 0.0, 0
+    if _autograd.wanted(x.feats, residual):
+        feats = _autograd.Dropout.apply(x.feats, residual, float(p), seed, int(offset))
+    else:
+        feats = _ext.dropout(x.feats, p, seed, offset, residual)
+    return x.replace(feats=feats)
 
 
 def layer_norm(x: SparseTensor, *, weight=None, bias=None, eps: float = 1e-5) -> SparseTensor:
-    """Layer normalisation of every sparse row over its channels (``ops/feature.py:196-210``)."""
+    """Layer normalisation of every sparse row over its channels (``ops/feature.py:196-210``).
+    Differentiable in ``x.feats``, ``weight`` and ``bias``."""
     if eps <= 0:
         raise ValueError('eps must be positive.')
+    if _autograd.wanted(x.feats, weight, bias):
+        return x.replace(feats=_autograd.RowNorm.apply(x.feats, weight, bias, float(eps), False))
     return x.replace(feats=_ext.row_norm(x.feats, weight, bias, eps, rms=False))
 
 
 def rms_norm(x: SparseTensor, *, weight=None, eps: float = 1e-5) -> SparseTensor:
-    """RMS normalisation of every sparse row (``ops/feature.py:214-225``)."""
+    """RMS normalisation of every sparse row (``ops/feature.py:214-225``). Differentiable in
+    ``x.feats`` and ``weight``."""
     if eps <= 0:
         raise ValueError('eps must be positive.')
+    if _autograd.wanted(x.feats, weight):
+        return x.replace(feats=_autograd.RowNorm.apply(x.feats, weight, None, float(eps), True))
     return x.replace(feats=_ext.row_norm(x.feats, weight, None, eps, rms=True))
 
 

@@ -1,0 +1,90 @@
+"""Refusals of the training and sequence operators that need no device: the C entry points
+check their arguments before any launch, and the Python layer before it touches a device."""
+
+import ctypes
+
+import pytest
+import torch
+
+from mlx_lattice_b200 import _ext, _native, nn, ops
+
+F32, F16 = 0, 1
+
+
+def _refused(code, text):
+    assert code == _native.LAT_INVALID_ARGUMENT
+    assert text in _native.last_error()
+
+
+def test_row_norm_entry_points_refuse_bad_arguments():
+    lib = _native.load()
+    buf = ctypes.c_void_p(4096)
+    _refused(lib.lat_row_norm_forward(2, 0, buf, 4, 8, 8, None, None, 1e-5, buf, buf, buf, None), 'float32 and float16')
+    _refused(lib.lat_row_norm_forward(F32, 0, buf, 4, 8, 8, None, None, 0.0, buf, buf, buf, None), 'eps must be positive')
+    _refused(lib.lat_row_norm_forward(F32, 0, buf, 4, 0, 8, None, None, 1e-5, buf, buf, buf, None), 'shape (N, C)')
+    _refused(lib.lat_row_norm_forward(F32, 0, buf, -1, 8, 8, None, None, 1e-5, buf, buf, buf, None), 'shape (N, C)')
+    _refused(lib.lat_row_norm_forward(F32, 1, buf, 4, 8, 8, None, buf, 1e-5, buf, None, buf, None), 'no bias')
+    _refused(lib.lat_row_norm_forward(F32, 0, buf, 4, 8, 8, None, None, 1e-5, buf, None, buf, None), 'statistics')
+    _refused(lib.lat_row_norm_backward(F32, 0, buf, 8, buf, 4, 8, 8, None, None, buf, buf, None, None, None, 0, None),
+             'statistics of the forward pass')
+    need = lib.lat_row_norm_backward_workspace_bytes(4, 8)
+    assert lib.lat_row_norm_backward(F32, 0, buf, 8, buf, 4, 8, 8, None, buf, buf, buf, buf, None, buf, need - 1,
+                                     None) == _native.LAT_WORKSPACE_TOO_SMALL
+    # nothing to do is no error, and touches no pointer
+    assert lib.lat_row_norm_forward(F32, 0, None, 0, 8, 8, None, None, 1e-5, None, None, None, None) == _native.LAT_OK
+
+
+def test_dropout_entry_point_refuses_bad_arguments():
+    lib = _native.load()
+    buf = ctypes.c_void_p(4096)
+    for p in (1.0, -0.1, float('nan')):
+        _refused(lib.lat_dropout(F32, buf, None, 8, p, 1, None, 0, buf, None), '0 <= p < 1')
+    _refused(lib.lat_dropout(3, buf, None, 8, 0.5, 1, None, 0, buf, None), 'float32 and float16')
+    _refused(lib.lat_dropout(F16, buf, None, -8, 0.5, 1, None, 0, buf, None), 'shape (N, C)')
+    _refused(lib.lat_dropout(F16, buf, None, 8, 0.5, 1, ctypes.c_void_p(4097), 0, buf, None), 'device seed')
+    assert lib.lat_dropout(F16, None, None, 0, 0.5, 1, None, 0, None, None) == _native.LAT_OK
+
+
+def test_recurrence_entry_points_refuse_bad_arguments():
+    lib = _native.load()
+    buf = ctypes.c_void_p(4096)
+
+    def forward(dtype=F32, rows=4, channels=8, offsets=buf, sequences=1, x=buf, stride=8, ws=None, ws_bytes=0):
+        return lib.lat_recurrence_forward(dtype, x, stride, buf, 8, rows, channels, offsets, sequences, None, 0, buf,
+                                          None, None, ws, ws_bytes, None, None)
+
+    _refused(forward(dtype=5), 'float32 and float16')
+    _refused(forward(rows=-1), 'shape (N, C)')
+    _refused(forward(rows=2 ** 31 - 1), 'shape (N, C)')
+    _refused(forward(channels=0), 'shape (N, C)')
+    _refused(forward(stride=-1), 'shape (N, C)')
+    _refused(forward(sequences=-1), 'offsets')
+    _refused(forward(offsets=None), 'offsets')
+    _refused(forward(offsets=None, sequences=0), 'offsets')
+    _refused(forward(x=None), 'shape (N, C)')
+    need = lib.lat_recurrence_workspace_bytes(300, 8)
+    assert forward(rows=300, ws=buf, ws_bytes=need - 1) == _native.LAT_WORKSPACE_TOO_SMALL
+    assert forward(rows=300) == _native.LAT_WORKSPACE_TOO_SMALL
+    assert forward(rows=0, x=None, offsets=None, sequences=0) == _native.LAT_OK
+    _refused(lib.lat_recurrence_backward(F32, buf, 8, None, buf, 8, buf, 8, 4, 8, buf, 1, None, 0, None, buf, buf, None,
+                                         None, 0, None, None), 'tile states')
+    _refused(lib.lat_recurrence_step(F32, buf, 8, buf, 8, None, 4, 8, buf, buf, None), 'state must have shape')
+    _refused(lib.lat_recurrence_step(F32, buf, 8, buf, 8, buf, 4, 0, buf, buf, None), 'shape (N, C)')
+    assert [lib.lat_recurrence_tiles(n) for n in (-1, 0, 1, 128, 129)] == [0, 0, 1, 1, 2]
+
+
+def test_host_tensors_are_refused():
+    x = torch.zeros((4, 8))
+    for call in (lambda: _ext.row_norm_forward(x, None, None, 1e-5, False),
+                 lambda: _ext.dropout(x, 0.5, 1),
+                 lambda: _ext.recurrence_forward(x, x, torch.zeros(2, dtype=torch.int32)),
+                 lambda: _ext.recurrence_step(x, x, x)):
+        with pytest.raises(RuntimeError, match='CUDA device'):
+            call()
+
+
+def test_module_arguments():
+    with pytest.raises(ValueError, match='0 <= p < 1'):
+        nn.Dropout(1.0)
+    assert nn.GatedRecurrence(reverse=True).reverse
+    assert {'gated_recurrence', 'gated_recurrence_step', 'sequence_offsets'} <= set(ops.__all__)
