@@ -510,10 +510,10 @@ int lat_dropout(
  * from its last row to its first. Rows outside all sequences give zeros. out [rows, channels]
  * is dense; final_state [sequences, channels] float32 (or NULL) is the h after the last row (an
  * empty sequence hands its initial state on). carries (NULL unless a backward pass follows):
- * float32 [lat_recurrence_tiles(rows), channels]. One pass; bitwise repeatable. A wait on
- * another block that runs out of its budget raises LAT_STATUS_WAIT_TIMEOUT. */
-size_t lat_recurrence_workspace_bytes(int32_t rows, int32_t channels);
-int32_t lat_recurrence_tiles(int32_t rows);
+ * float32 [lat_recurrence_carry_rows(rows), channels], the h before every eighth row. Bitwise
+ * repeatable. */
+size_t lat_recurrence_workspace_bytes(int32_t dtype, int32_t rows, int32_t channels);
+int32_t lat_recurrence_carry_rows(int32_t rows);
 int lat_recurrence_forward(
     int32_t dtype, const void* feats, int64_t feat_row_stride, const void* gate, int64_t gate_row_stride,
     int32_t rows, int32_t channels, const int32_t* offsets, int32_t sequences, const float* initial_state,

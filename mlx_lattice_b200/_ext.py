@@ -1285,9 +1285,9 @@ def recurrence_forward(feats, gate, offsets, initial_state=None, reverse: bool =
     out = torch.empty((rows, channels), dtype=feats.dtype, device=device)
     lib = _lib()
     final = torch.empty((sequences, channels), dtype=torch.float32, device=device) if want_state else None
-    carries = (torch.empty((lib.lat_recurrence_tiles(rows), channels), dtype=torch.float32, device=device)
+    carries = (torch.empty((lib.lat_recurrence_carry_rows(rows), channels), dtype=torch.float32, device=device)
                if want_carries else None)
-    ws = _workspace(lib.lat_recurrence_workspace_bytes(rows, channels), device)
+    ws = _workspace(lib.lat_recurrence_workspace_bytes(dtype, rows, channels), device)
     with torch.cuda.device(device):
         check(lib.lat_recurrence_forward(
             dtype, _ptr(feats), stride, _ptr(gate), gate_stride, rows, channels, _ptr(offsets), sequences,
@@ -1309,11 +1309,11 @@ def recurrence_backward(grad, grad_final, feats, gate, offsets, initial_state, r
     initial_state = _state_arg(initial_state, 'initial_state', sequences, channels, device)
     grad_final = _state_arg(grad_final, 'grad_final', sequences, channels, device)
     lib = _lib()
-    carries = _state_arg(carries, 'carries', lib.lat_recurrence_tiles(rows), channels, device)
+    carries = _state_arg(carries, 'carries', lib.lat_recurrence_carry_rows(rows), channels, device)
     grad_feats = torch.empty((rows, channels), dtype=feats.dtype, device=device)
     grad_gate = torch.empty((rows, channels), dtype=feats.dtype, device=device)
     grad_initial = torch.empty((sequences, channels), dtype=torch.float32, device=device) if want_initial else None
-    ws = _workspace(lib.lat_recurrence_workspace_bytes(rows, channels), device)
+    ws = _workspace(lib.lat_recurrence_workspace_bytes(dtype, rows, channels), device)
     with torch.cuda.device(device):
         check(lib.lat_recurrence_backward(
             dtype, _ptr(grad), grad_stride, _ptr(grad_final), _ptr(feats), stride, _ptr(gate), gate_stride, rows,

@@ -115,8 +115,8 @@ SIGNATURES = {
     'lat_row_norm_backward': (
         I, [I, I, P, c_int64, P, c_int64, I, c_int64, P, P, P, P, P, P, P, c_size_t, P]),
     'lat_dropout': (I, [I, P, P, c_int64, c_double, c_uint64, P, c_uint64, P, P]),
-    'lat_recurrence_workspace_bytes': (c_size_t, [I, I]),
-    'lat_recurrence_tiles': (I, [I]),
+    'lat_recurrence_workspace_bytes': (c_size_t, [I, I, I]),
+    'lat_recurrence_carry_rows': (I, [I]),
     'lat_recurrence_forward': (
         I, [I, P, c_int64, P, c_int64, I, I, P, I, P, I, P, P, P, P, c_size_t, P, P]),
     'lat_recurrence_backward': (

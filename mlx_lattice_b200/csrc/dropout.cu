@@ -57,17 +57,21 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(
     if (seed_device != nullptr) {
         seed = __ldg(seed_device);
     }
+    // the loads are on their way while the words are computed
+    const bool whole = first + V <= total;
+    Pack<T, V> in, add, y;
+    if (whole) {
+        in = load_pack<T, V>(x + first);
+        if (residual != nullptr) {
+            add = load_pack<T, V>(residual + first);
+        }
+    }
     Words words[V / 4];
 #pragma unroll
     for (int q = 0; q < V / 4; ++q) {
         words[q] = philox(static_cast<unsigned long long>(first) / 4 + q, offset, seed);
     }
-    if (first + V <= total) {
-        const Pack<T, V> in = load_pack<T, V>(x + first);
-        Pack<T, V> add, y;
-        if (residual != nullptr) {
-            add = load_pack<T, V>(residual + first);
-        }
+    if (whole) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float v = words[i / 4].w[i % 4] >= threshold ? in.get(i) * scale : 0.0f;

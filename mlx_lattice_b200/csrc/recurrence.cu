@@ -7,29 +7,24 @@
 //   dh_t = dy_t + a_{t+1} dh_{t+1}  (+ dfinal at the last row)
 //   dx_t = (1 - a_t) dh_t,  dz_t = a_t (1 - a_t) dh_t (h_{t-1} - x_t),  dinitial = a_1 dh_1
 //
-// Both directions are scans over affine maps h -> A h + H, which compose associatively. A
-// block owns a tile of 128 rows and a slab of channels, holds it in registers, and a thread
-// walks 8 rows of a few channels. The maps of the 16 row segments of a tile are composed in
-// shared memory; tiles are chained over the rows through the workspace in one pass, so every
-// input is read once and every output written once. What bounds it is the memory.
-//
-// The chain has a fixed shape: a tile composes the maps of the earlier tiles of its group of
-// 16, the maps of the earlier groups of its supergroup of 16 groups, and the state at the
-// start of the supergroup, always in this order. Results therefore do not depend on which
-// block came first, and are bitwise repeatable. Blocks take tiles in ticket order, so a tile
-// only waits for tiles that already run; every wait has a clock budget.
-//
-// A record of the chain is one 64-bit word, (A, H) or (0, h): it is written and read whole,
-// so it needs no flag beside it. All ones (no arithmetic result has these bits in its low
-// half) means "not yet written".
+// Both directions are scans over affine maps h -> A h + H, which compose associatively. The
+// rows are cut into tiles of 64; a thread walks one tile for eight bytes of channels. Three
+// kernels:
+//   maps:   the map (A, H) of every tile, and for a group of tiles (a block) the maps of the
+//           tiles before each one in the group and of the whole group
+//   scan:   the state that reaches every group, from the groups' maps
+//   apply:  the state that reaches a tile is its map within the group applied to the group's
+//           state; walk the tile again from there and write
+// Nothing waits for anything inside a kernel, and every sum has a fixed order: results are
+// bitwise repeatable.
 //
 // A row that starts a sequence cuts the chain. Its map ignores the incoming h altogether
 // (marked by A = -1, and selected, not multiplied by zero: a NaN or an infinity of one
 // sequence does not reach the next). Rows outside all sequences give zeros.
 //
-// The backward pass recomputes h from the state at the start of each tile, which the forward
-// pass leaves in float32 (4 / (128 * element size) of the features): it reads x, z, dy and
-// writes dx, dz, and its h is not rounded to the feature type.
+// The backward pass recomputes h from the state at the start of every eight rows, which the
+// forward pass leaves in float32: it reads x, z, dy and writes dx, dz, and its h is not rounded
+// to the feature type.
 #include <algorithm>
 
 #include "common.cuh"
@@ -39,50 +34,11 @@ namespace lat {
 
 namespace {
 
-constexpr int kSegments = 16;
-constexpr int kSegmentRows = 8;
-constexpr int kTileRows = kSegments * kSegmentRows;
-constexpr int kGroup = 16;                    // tiles of a group, groups of a supergroup
+constexpr int kTileRows = 64;
+constexpr int kThreads = 256;
 constexpr float kReset = -1.0f;
-
-struct Chain {
-    unsigned long long* tiles;   // [tiles][channels]    (A, H)
-    unsigned long long* groups;  // [groups][channels]   (A, H)
-    unsigned long long* states;  // [supergroups][channels]  (0, h at its first tile)
-    int* ticket;                 // -1 before the first block
-    long long budget;
-    int32_t* status;
-};
-
-__device__ __forceinline__ unsigned long long record(float low, float high) {
-    uint32_t bits = __float_as_uint(low);
-    bits = bits == 0xFFFFFFFFu ? 0x7FFFFFFFu : bits;
-    return (static_cast<unsigned long long>(__float_as_uint(high)) << 32) | bits;
-}
-
-__device__ __forceinline__ unsigned long long read_record(const unsigned long long* p) {
-    unsigned long long v;
-    asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
-    return v;
-}
-
-__device__ __forceinline__ void write_record(unsigned long long* p, unsigned long long v) {
-    asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
-}
-
-__device__ __forceinline__ float2 wait_record(const unsigned long long* p, unsigned long long v, const Chain& chain) {
-    if (static_cast<uint32_t>(v) == 0xFFFFFFFFu) {
-        const long long start = clock64();
-        while (static_cast<uint32_t>(v = read_record(p)) == 0xFFFFFFFFu) {
-            if (clock64() - start > chain.budget) {
-                raise_status(chain.status, LAT_STATUS_WAIT_TIMEOUT);
-                v = 0;
-                break;
-            }
-        }
-    }
-    return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
-}
+constexpr int kCarryRows = 8;                 // rows from one kept state to the next
+template <typename T> constexpr int kWide = 8 / static_cast<int>(sizeof(T));   // channels of a thread
 
 // later after earlier, as maps
 __device__ __forceinline__ float2 compose(float2 earlier, float2 later) {
@@ -94,67 +50,6 @@ __device__ __forceinline__ float2 compose(float2 earlier, float2 later) {
 
 __device__ __forceinline__ float apply(float2 map, float h) {
     return map.x == kReset ? map.y : fmaf(map.x, h, map.y);
-}
-
-// Map of `count` consecutive records in order; eight loads in flight.
-__device__ __forceinline__ float2 compose_records(
-    const unsigned long long* first, int count, int stride, const Chain& chain
-) {
-    float2 map = make_float2(1.0f, 0.0f);
-    for (int base = 0; base < count; base += 8) {
-        unsigned long long raw[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            raw[i] = base + i < count ? read_record(first + static_cast<size_t>(base + i) * stride) : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (base + i < count) {
-                map = compose(map, wait_record(first + static_cast<size_t>(base + i) * stride, raw[i], chain));
-            }
-        }
-    }
-    return map;
-}
-
-// The state that reaches tile `tile` (in chain order) in channel `c`, given the tile's own
-// map, which is published for the tiles behind it. `needed` is false when the tile's first
-// row cuts the chain.
-__device__ __forceinline__ float chain_through(
-    const Chain& chain, int tile, int tiles, int channels, int c, float2 own, bool needed
-) {
-    if (tile + 1 < tiles) {
-        write_record(chain.tiles + static_cast<size_t>(tile) * channels + c, record(own.x, own.y));
-    }
-    const int group = tile / kGroup, member = tile % kGroup;
-    const int super = group / kGroup, group_member = group % kGroup;
-    const bool last = member == kGroup - 1, last_group = last && group_member == kGroup - 1;
-    const bool cut = own.x == kReset;
-    float2 near = make_float2(1.0f, 0.0f);
-    if (needed || (last && !cut)) {
-        near = compose_records(chain.tiles + static_cast<size_t>(group) * kGroup * channels + c, member, channels, chain);
-    }
-    if (last && tile + 1 < tiles) {
-        const float2 map = compose(near, own);
-        write_record(chain.groups + static_cast<size_t>(group) * channels + c, record(map.x, map.y));
-    }
-    float h = 0.0f;
-    if (needed || (last_group && !cut)) {
-        if (near.x != kReset) {
-            const float2 far = compose_records(
-                chain.groups + static_cast<size_t>(super) * kGroup * channels + c, group_member, channels, chain);
-            if (far.x != kReset && super > 0) {
-                const unsigned long long* state = chain.states + static_cast<size_t>(super) * channels + c;
-                h = wait_record(state, read_record(state), chain).y;
-            }
-            h = apply(far, h);
-        }
-        h = apply(near, h);
-    }
-    if (last_group && tile + 1 < tiles) {
-        write_record(chain.states + static_cast<size_t>(super + 1) * channels + c, record(0.0f, apply(own, h)));
-    }
-    return h;
 }
 
 // Rows and sequences in the order of time: row i is row rows - 1 - i of the arrays when the
@@ -173,59 +68,118 @@ struct Order {
     __device__ __forceinline__ int sequence(int j) const { return reverse ? sequences - 1 - j : j; }
 };
 
-// What the rows of a tile are: `head` the sequence that starts there, -1 a row that follows
-// another, -2 a row outside all sequences; `tail` the sequence that ends there or -1.
-struct RowTable {
-    int head[kTileRows];
-    int tail[kTileRows];
+// ---- arithmetic on pairs of channels: one instruction for two floats ----------------------
+
+struct alignas(8) Pair {
+    float x, y;
 };
 
-__device__ __forceinline__ void fill_rows(RowTable& table, const Order& order, int first, int32_t* status) {
-    const int begin = order.begin(0), end = order.begin(order.sequences);
-    for (int i = threadIdx.x; i < kTileRows; i += blockDim.x) {
-        table.head[i] = first + i < begin || first + i >= end ? -2 : -1;
-        table.tail[i] = -1;
-    }
-    // the first sequence that ends behind the tile's first row
-    int low = 0, high = order.sequences;
-    while (low < high) {
-        const int mid = (low + high) >> 1;
-        if (order.begin(mid + 1) > first) {
-            high = mid;
-        } else {
-            low = mid + 1;
-        }
-    }
-    __syncthreads();
-    for (int j = low + static_cast<int>(threadIdx.x); j < order.sequences; j += blockDim.x) {
-        const int b = order.begin(j) - first, e = order.begin(j + 1) - first;
-        if (e < b) {
+__device__ __forceinline__ Pair both(float v) { return {v, v}; }
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+    Pair d;
+    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+    Pair d;
+    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
+        "fma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
+        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ Pair minus(Pair a, Pair b) { return fma(b, both(-1.0f), a); }   // a - b, rounded once
+
+__device__ __forceinline__ float exp2_fast(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+// one unit in the last place; zero beyond 2^126
+__device__ __forceinline__ float reciprocal(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+constexpr float kMinusLog2E = -1.4426950408889634f;
+
+// exp(-z). sigmoid(z) = 1 / (1 + exp(-z)) and sigmoid(-z) = exp(-z) sigmoid(z), each to full
+// relative precision as long as exp(-z) stays below 2^126, where the reciprocal becomes zero.
+// That is z > -87.336; below, sigmoid(z) is less than the smallest normal float anyway.
+constexpr float kLowestGate = -87.33f;
+
+__device__ __forceinline__ Pair exp_minus(Pair z) {
+    const Pair t = z * both(kMinusLog2E);
+    return {exp2_fast(t.x), exp2_fast(t.y)};
+}
+__device__ __forceinline__ Pair sigmoid_from(Pair odds) {
+    const Pair d = odds + both(1.0f);
+    return {reciprocal(d.x), reciprocal(d.y)};
+}
+__device__ __forceinline__ float sigmoid_gate(float z) { return reciprocal(1.0f + exp2_fast(z * kMinusLog2E)); }
+
+// Offsets that fall are reported; the threads of the grid look at them in turn.
+__device__ __forceinline__ void check_offsets(const Order& order, int32_t* status) {
+    const long long threads = static_cast<long long>(gridDim.x) * blockDim.x;
+    for (long long j = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; j < order.sequences; j += threads) {
+        if (__ldg(order.offsets + j + 1) < __ldg(order.offsets + j)) {
             raise_status(status, LAT_STATUS_BAD_INDEX);
         }
-        if (b >= kTileRows) {
-            break;
-        }
-        if (e > b) {
-            if (b >= 0) {
-                table.head[b] = j;
-            }
-            if (e >= 1 && e <= kTileRows) {
-                table.tail[e - 1] = j;
-            }
-        }
     }
-    __syncthreads();
 }
 
-__device__ __forceinline__ float sigmoid_gate(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
+// The sequence that holds a row or, for a row outside all of them, the next one; in the order of
+// time.
+struct Cursor {
+    int j, begin, end;
 
-// sigmoid(z) and sigmoid(-z), each to full relative precision; z is bounded below so that
-// exp(-z) stays finite (a NaN passes)
-__device__ __forceinline__ void sigmoid_pair(float z, float& a, float& rest) {
-    const float e = __expf(z < -80.0f ? 80.0f : -z);
-    a = __fdividef(1.0f, 1.0f + e);
-    rest = e * a;
-}
+    __device__ __forceinline__ void settle(const Order& order) {
+        while (j < order.sequences) {
+            begin = order.begin(j);
+            end = order.begin(j + 1);
+            if (end > begin) {
+                return;
+            }
+            ++j;   // no rows
+        }
+        begin = end = 0x7fffffff;
+    }
+
+    // the first sequence that ends behind row `first`
+    __device__ __forceinline__ void seek(const Order& order, int first) {
+        int low = 0, high = order.sequences;
+        while (low < high) {
+            const int mid = (low + high) >> 1;
+            if (order.begin(mid + 1) > first) {
+                high = mid;
+            } else {
+                low = mid + 1;
+            }
+        }
+        j = low;
+        settle(order);
+    }
+
+    __device__ __forceinline__ void next(const Order& order) {
+        ++j;
+        settle(order);
+    }
+
+    // no sequence starts or ends among these rows, which all belong to this one
+    __device__ __forceinline__ bool covers(int first, int rows) const { return begin < first && end > first + rows; }
+};
 
 template <typename T> struct ScanArgs {
     const T* x;
@@ -234,321 +188,595 @@ template <typename T> struct ScanArgs {
     long long x_stride, z_stride, dy_stride;
     Order order;
     int channels;
-    int slabs;
+    int slabs;              // of kWide * lanes channels
+    int lanes;              // threads across a slab, eight bytes each
     int tiles;
     const float* initial;   // [sequences][channels] or null
-    float* carries;         // [tiles][channels] or null: h that reaches each tile
+    float2* maps;           // [tiles][channels] of the tiles before in the group
+    float2* groups;         // [groups][channels]
+    float* states;          // [groups][channels] that reach the groups, or null: zero
+    float* carries;         // [batches][channels] or null: h before each batch of rows
     T* h;
     float* final;           // [sequences][channels] or null
     const float* dfinal;    // [sequences][channels] or null
     T* dx;
     T* dz;
     float* dinitial;        // [sequences][channels] or null
-    Chain chain;
+    int32_t* status;
 };
 
-__device__ __forceinline__ int take_ticket(int* ticket) {
-    __shared__ int taken;
-    if (threadIdx.x == 0) {
-        taken = atomicAdd(ticket, 1) + 1;
+// The channels of a thread in one row, as they are stored ...
+template <typename T> struct alignas(8) Stored {
+    T v[kWide<T>];
+};
+
+// ... and as float pairs.
+template <typename T> struct Row {
+    static constexpr int kPairs = kWide<T> / 2;
+    Pair v[kPairs];
+
+    static __device__ __forceinline__ Row filled(float value) {
+        Row out;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            out.v[i] = both(value);
+        }
+        return out;
     }
-    __syncthreads();
-    return taken;
-}
 
-// Block: Q threads across the slab (V channels each) times kSegments down the tile.
-template <typename T, int V, int Q>
-__global__ void __launch_bounds__(Q * kSegments) recurrence_forward_kernel(ScanArgs<T> p) {
-    constexpr int C = Q * V;
-    __shared__ RowTable table;
-    __shared__ float2 maps[kSegments][C];
-    const int id = p.tiles > 1 ? take_ticket(p.chain.ticket) : static_cast<int>(blockIdx.x);
-    const int tile = id / p.slabs, slab = id - tile * p.slabs;
-    const int first = tile * kTileRows;
-    const int segment = threadIdx.x / Q;
-    const int in_slab = (threadIdx.x % Q) * V;
-    const int c = slab * C + in_slab;
-    const bool in = c < p.channels;
-    const int begin = first + segment * kSegmentRows;
+    static __device__ __forceinline__ Row from(const Stored<T>& raw) {
+        Row out;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            if constexpr (sizeof(T) == 2) {
+                const float2 f = __half22float2(__halves2half2(raw.v[2 * i], raw.v[2 * i + 1]));
+                out.v[i] = {f.x, f.y};
+            } else {
+                out.v[i] = {raw.v[2 * i], raw.v[2 * i + 1]};
+            }
+        }
+        return out;
+    }
 
-    Pack<T, V> x[kSegmentRows];
-    float a[kSegmentRows][V];
+    __device__ __forceinline__ float get(int i) const { return i % 2 == 0 ? v[i / 2].x : v[i / 2].y; }
+    __device__ __forceinline__ void set(int i, float value) { (i % 2 == 0 ? v[i / 2].x : v[i / 2].y) = value; }
+};
+
+// A thread's place: its tile and its channels c .. c + count - 1, at most kWide. Tiles are
+// numbered in the order of the chain (`place`): of time, or backwards in time for the gradient.
+// Whole: channels come in full eights of bytes and can be moved at once.
+template <typename T, bool Whole, bool Backward> struct Walk {
+    int place, tile, c, count;
+    long long row_step;   // from a row to the next one, in rows of an array
+
+    __device__ __forceinline__ Walk(const ScanArgs<T>& p, int block) {
+        const int group = block / p.slabs, slab = block - group * p.slabs;
+        place = group * (kThreads / p.lanes) + static_cast<int>(threadIdx.x) / p.lanes;
+        tile = Backward ? p.tiles - 1 - place : place;
+        c = (slab * p.lanes + static_cast<int>(threadIdx.x) % p.lanes) * kWide<T>;
+        count = place < p.tiles ? min(max(p.channels - c, 0), kWide<T>) : 0;
+        row_step = p.order.reverse ? -1 : 1;
+    }
+
+    // to: the thread's first channel in the row
+    __device__ __forceinline__ void store(T* to, const Row<T>& value) const {
+        Stored<T> raw;
+        if constexpr (sizeof(T) == 2) {
 #pragma unroll
-    for (int r = 0; r < kSegmentRows; ++r) {
-        const bool live = in && begin + r < p.order.rows;
-        const size_t row = live ? p.order.row(begin + r) : 0;
-        x[r] = live ? load_pack<T, V>(p.x + row * p.x_stride + c) : zero_pack<T, V>();
-        const Pack<T, V> z = live ? load_pack<T, V>(p.z + row * p.z_stride + c) : zero_pack<T, V>();
+            for (int i = 0; i < Row<T>::kPairs; ++i) {
+                const __half2 h = __floats2half2_rn(value.v[i].x, value.v[i].y);
+                raw.v[2 * i] = __low2half(h);
+                raw.v[2 * i + 1] = __high2half(h);
+            }
+        } else {
+            raw.v[0] = value.v[0].x;
+            raw.v[1] = value.v[0].y;
+        }
+        if constexpr (Whole) {
+            *reinterpret_cast<Stored<T>*>(to) = raw;
+        } else {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            a[r][i] = z.get(i);
+            for (int i = 0; i < kWide<T>; ++i) {
+                if (i < count) {
+                    to[i] = raw.v[i];
+                }
+            }
         }
     }
-    fill_rows(table, p.order, first, p.chain.status);
 
-    float prod[V], h[V];
+    // Row `row` of a float array [..][channels], or zeros without one.
+    __device__ __forceinline__ Row<T> state(const float* from, long long row, int channels) const {
+        Row<T> out = Row<T>::filled(0.0f);
+        if (from != nullptr) {
+            from += row * channels + c;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        prod[i] = 1.0f;
-        h[i] = 0.0f;
+            for (int i = 0; i < kWide<T>; ++i) {
+                if (Whole || i < count) {
+                    out.set(i, from[i]);
+                }
+            }
+        }
+        return out;
     }
+
+    __device__ __forceinline__ void store_state(float* to, long long row, int channels, const Row<T>& value) const {
+        if (to != nullptr) {
+            to += row * channels + c;
+            if constexpr (Whole) {
+                Pack<float, kWide<T>> out;
+#pragma unroll
+                for (int i = 0; i < kWide<T>; ++i) {
+                    out.v[i] = value.get(i);
+                }
+                store_pack<float, kWide<T>>(to, out);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kWide<T>; ++i) {
+                    if (i < count) {
+                        to[i] = value.get(i);
+                    }
+                }
+            }
+        }
+    }
+};
+
+// Rows on their way from the arrays to a thread: a ring of stages in shared memory, each with
+// Rows rows of every array, filled by asynchronous copies of eight bytes. A thread copies what it
+// reads itself, so nothing is synchronised, and the bytes in flight (the memory needs some 50 KB
+// of them per SM) cost no registers.
+template <typename T, bool Whole, int Arrays, int Rows, int Stages> struct Ring {
+    static constexpr int kBytes = Stages * Arrays * Rows * kThreads * 8;
+
+    __device__ __forceinline__ Stored<T>* slot(int stage, int array, int row) const {
+        extern __shared__ __align__(16) unsigned char ring[];
+        return reinterpret_cast<Stored<T>*>(ring) + ((stage * Arrays + array) * Rows + row) * kThreads + threadIdx.x;
+    }
+
+    // Rows first .. first + Rows - 1; zeros from row `end` on and for channels that do not exist.
+    template <typename W>
+    __device__ __forceinline__ void fetch(
+        const W& walk, int stage, int array, const T* from, long long stride, const Order& order, int first, int end
+    ) const {
+        const T* at = from + order.row(first) * stride + walk.c;
+        const long long step = walk.row_step * stride;
+        if (Whole && first + Rows <= end) {
+            const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot(stage, array, 0)));
+#pragma unroll
+            for (int r = 0; r < Rows; ++r) {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to + r * kThreads * 8), "l"(at) : "memory");
+                at += step;
+            }
+        } else {
+            for (int r = 0; r < Rows; ++r) {
+                Stored<T> raw;
+#pragma unroll
+                for (int i = 0; i < kWide<T>; ++i) {
+                    raw.v[i] = first + r < end && i < walk.count ? at[i] : narrow<T>(0.0f);
+                }
+                *slot(stage, array, r) = raw;
+                at += step;
+            }
+        }
+    }
+
+    // ends a stage's fetches
+    __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    // the oldest stage is there; the ones behind it may still be on their way
+    __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(Stages - 2) : "memory"); }
+
+    __device__ __forceinline__ Row<T> row(int stage, int array, int r) const { return Row<T>::from(*slot(stage, array, r)); }
+};
+
+// Maps of the tiles of a group -> the maps before each tile in the group, and the group's map.
+template <typename T, typename W>
+__device__ __forceinline__ void share_maps(
+    const ScanArgs<T>& p, const W& walk, bool cut, const Row<T>& product, const Row<T>& sum
+) {
+    constexpr int N = kWide<T>;
+    __shared__ float2 maps[N * kThreads];   // [tiles of the group][N * lanes]
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        maps[N * threadIdx.x + i] = make_float2(cut ? kReset : product.get(i), sum.get(i));
+    }
+    __syncthreads();
+    const int width = N * p.lanes, tiles = kThreads / p.lanes;
+    if (static_cast<int>(threadIdx.x) < width) {
+        float2 all = make_float2(1.0f, 0.0f);
+#pragma unroll 4
+        for (int k = 0; k < tiles; ++k) {
+            const float2 own = maps[k * width + threadIdx.x];
+            maps[k * width + threadIdx.x] = all;
+            all = compose(all, own);
+        }
+        const int group = blockIdx.x / p.slabs;
+        const int c = (blockIdx.x - group * p.slabs) * width + threadIdx.x;
+        if (c < p.channels) {
+            p.groups[static_cast<size_t>(group) * p.channels + c] = all;
+        }
+    }
+    __syncthreads();
+    float2* to = p.maps + static_cast<size_t>(walk.place) * p.channels + walk.c;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        if (i < walk.count) {
+            to[i] = maps[N * threadIdx.x + i];
+        }
+    }
+}
+
+// The state that reaches the thread's tile.
+template <typename T, typename W>
+__device__ __forceinline__ Row<T> reaching_state(const ScanArgs<T>& p, const W& walk, int block) {
+    Row<T> out = Row<T>::filled(0.0f);
+    if (p.maps != nullptr) {
+        const int group = block / p.slabs;
+        const float* state = p.states == nullptr ? nullptr : p.states + static_cast<size_t>(group) * p.channels + walk.c;
+        const float2* map = p.maps + static_cast<size_t>(walk.place) * p.channels + walk.c;
+#pragma unroll
+        for (int i = 0; i < kWide<T>; ++i) {
+            if (i < walk.count) {
+                out.set(i, apply(map[i], state == nullptr ? 0.0f : state[i]));
+            }
+        }
+    }
+    return out;
+}
+
+template <bool Value> struct Flag {
+    static constexpr bool value = Value;
+};
+
+// One row of the recurrence.
+template <typename T>
+__device__ __forceinline__ void advance(Row<T>& h, const Row<T>& a, const Row<T>& x) {
+#pragma unroll
+    for (int i = 0; i < Row<T>::kPairs; ++i) {
+        h.v[i] = fma(a.v[i], h.v[i], minus(both(1.0f), a.v[i]) * x.v[i]);
+    }
+}
+
+template <typename T> __device__ __forceinline__ Row<T> gates(const Row<T>& z) {
+    Row<T> a;
+#pragma unroll
+    for (int i = 0; i < Row<T>::kPairs; ++i) {
+        a.v[i] = sigmoid_from(exp_minus(z.v[i]));
+    }
+    return a;
+}
+
+constexpr int kRingRows = 4, kRingStages = 4;
+
+template <typename T, bool Whole>
+__global__ void __launch_bounds__(kThreads, 3) recurrence_maps_kernel(ScanArgs<T> p) {
+    constexpr int R = kRingRows, S = kRingStages;
+    const Walk<T, Whole, false> walk(p, blockIdx.x);
+    const Ring<T, Whole, 2, R, S> ring;
+    Row<T> prod = Row<T>::filled(1.0f), h = Row<T>::filled(0.0f);
     bool cut = false;
-#pragma unroll
-    for (int r = 0; r < kSegmentRows; ++r) {
-        const int head = table.head[segment * kSegmentRows + r];
-        if (head != -1) {
-            cut = true;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                h[i] = head >= 0 && in && p.initial != nullptr
-                           ? p.initial[static_cast<size_t>(p.order.sequence(head)) * p.channels + c + i]
-                           : 0.0f;
+    if (walk.count > 0) {
+        const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
+        const auto fetch = [&](int row, int stage) {
+            if (row < end) {
+                ring.fetch(walk, stage, 0, p.x, p.x_stride, p.order, row, end);
+                ring.fetch(walk, stage, 1, p.z, p.z_stride, p.order, row, end);
             }
+            ring.commit();
+        };
+#pragma unroll
+        for (int s = 0; s < S - 1; ++s) {
+            fetch(first + s * R, s);
         }
+        Cursor cursor;
+        cursor.seek(p.order, first);
+        int stage = 0;
+#pragma unroll 1
+        for (int row = first; row < end; row += R) {
+            ring.wait();
+            fetch(row + (S - 1) * R, (stage + S - 1) % S);
+            const auto scan = [&](auto marked) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            a[r][i] = sigmoid_gate(a[r][i]);
-            prod[i] *= a[r][i];
-            h[i] = fmaf(a[r][i], h[i], (1.0f - a[r][i]) * x[r].get(i));
-            if (head == -2) {
-                h[i] = 0.0f;
+                for (int r = 0; r < R; ++r) {
+                    if (decltype(marked)::value && row + r < cursor.begin) {
+                        cut = true;
+                        h = Row<T>::filled(0.0f);
+                        continue;
+                    }
+                    if (decltype(marked)::value && row + r == cursor.begin) {
+                        cut = true;
+                        h = walk.state(p.initial, p.order.sequence(cursor.j), p.channels);
+                    }
+                    const Row<T> a = gates<T>(ring.row(stage, 1, r));
+#pragma unroll
+                    for (int i = 0; i < Row<T>::kPairs; ++i) {
+                        prod.v[i] = prod.v[i] * a.v[i];
+                    }
+                    advance<T>(h, a, ring.row(stage, 0, r));
+                    if (decltype(marked)::value && row + r == cursor.end - 1) {
+                        cursor.next(p.order);
+                    }
+                }
+            };
+            if (cursor.covers(row, R)) {
+                scan(Flag<false>{});
+            } else {
+                scan(Flag<true>{});
             }
+            stage = (stage + 1) % S;
         }
     }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        maps[segment][in_slab + i] = make_float2(cut ? kReset : prod[i], h[i]);
-    }
-    __syncthreads();
-    if (threadIdx.x < C) {
-        const int channel = slab * C + threadIdx.x;
-        float2 own = make_float2(1.0f, 0.0f);
-#pragma unroll
-        for (int s = 0; s < kSegments; ++s) {
-            own = compose(own, maps[s][threadIdx.x]);
-        }
-        float state = 0.0f;
-        if (channel < p.channels) {
-            if (p.tiles > 1) {
-                state = chain_through(p.chain, tile, p.tiles, p.channels, channel, own, table.head[0] == -1);
-            }
-            if (p.carries != nullptr) {
-                p.carries[static_cast<size_t>(tile) * p.channels + channel] = state;
-            }
-        }
-        for (int s = 0; s < kSegments; ++s) {
-            const float2 map = maps[s][threadIdx.x];
-            maps[s][threadIdx.x].y = state;
-            state = apply(map, state);
-        }
-    }
-    __syncthreads();
-    if (!in) {
+    share_maps<T>(p, walk, cut, prod, h);
+}
+
+template <typename T, bool Whole>
+__global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<T> p) {
+    constexpr int R = kRingRows, S = kRingStages;
+    // the last tiles first: the maps kernel read them last
+    const int block = gridDim.x - 1 - blockIdx.x;
+    const Walk<T, Whole, false> walk(p, block);
+    const Ring<T, Whole, 2, R, S> ring;
+    check_offsets(p.order, p.status);
+    if (walk.count == 0) {
         return;
     }
+    const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
+    const auto fetch = [&](int row, int stage) {
+        if (row < end) {
+            ring.fetch(walk, stage, 0, p.x, p.x_stride, p.order, row, end);
+            ring.fetch(walk, stage, 1, p.z, p.z_stride, p.order, row, end);
+        }
+        ring.commit();
+    };
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        h[i] = maps[segment][in_slab + i].y;
+    for (int s = 0; s < S - 1; ++s) {
+        fetch(first + s * R, s);
     }
-#pragma unroll
-    for (int r = 0; r < kSegmentRows; ++r) {
-        if (begin + r >= p.order.rows) {
-            break;
+    Row<T> h = reaching_state<T>(p, walk, block);
+    Cursor cursor;
+    cursor.seek(p.order, first);
+    const long long down = walk.row_step * p.channels;
+    T* out = p.h + static_cast<long long>(p.order.row(first)) * p.channels + walk.c;
+    int stage = 0;
+#pragma unroll 1
+    for (int row = first; row < end; row += R) {
+        ring.wait();
+        fetch(row + (S - 1) * R, (stage + S - 1) % S);
+        if (row % kCarryRows == 0) {
+            walk.store_state(p.carries, row / kCarryRows, p.channels, h);
         }
-        const int head = table.head[segment * kSegmentRows + r], tail = table.tail[segment * kSegmentRows + r];
-        if (head >= 0) {
+        const auto write = [&](auto marked) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                h[i] = p.initial != nullptr
-                           ? p.initial[static_cast<size_t>(p.order.sequence(head)) * p.channels + c + i]
-                           : 0.0f;
+            for (int r = 0; r < R; ++r) {
+                if (decltype(marked)::value && row + r >= end) {
+                    break;
+                }
+                if (decltype(marked)::value && row + r == cursor.begin) {
+                    h = walk.state(p.initial, p.order.sequence(cursor.j), p.channels);
+                }
+                advance<T>(h, gates<T>(ring.row(stage, 1, r)), ring.row(stage, 0, r));
+                if (decltype(marked)::value && row + r < cursor.begin) {
+                    h = Row<T>::filled(0.0f);
+                }
+                walk.store(out, h);
+                out += down;
+                if (decltype(marked)::value && row + r == cursor.end - 1) {
+                    walk.store_state(p.final, p.order.sequence(cursor.j), p.channels, h);
+                    cursor.next(p.order);
+                }
             }
+        };
+        if (cursor.covers(row, R)) {
+            write(Flag<false>{});
+        } else {
+            write(Flag<true>{});
         }
-        Pack<T, V> y;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            h[i] = fmaf(a[r][i], h[i], (1.0f - a[r][i]) * x[r].get(i));
-            if (head == -2) {
-                h[i] = 0.0f;
-            }
-            y.set(i, h[i]);
-        }
-        store_pack<T, V>(p.h + static_cast<size_t>(p.order.row(begin + r)) * p.channels + c, y);
-        if (tail >= 0 && p.final != nullptr) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                p.final[static_cast<size_t>(p.order.sequence(tail)) * p.channels + c + i] = h[i];
-            }
-        }
+        stage = (stage + 1) % S;
     }
 }
 
-// The tiles in falling order. e_t = a_t dh_t is what a row hands to the row before it:
-// e_t = a_t e_{t+1} + a_t dy_t, the same kind of map with the same product of gates.
-template <typename T, int V, int Q>
-__global__ void __launch_bounds__(Q * kSegments) recurrence_backward_kernel(ScanArgs<T> p) {
-    constexpr int C = Q * V;
-    __shared__ RowTable table;
-    __shared__ float2 maps[kSegments][C];    // forward maps, then h at the start of a segment
-    __shared__ float2 flows[kSegments][C];   // backward maps, then e at the end of a segment
-    const int id = p.tiles > 1 ? take_ticket(p.chain.ticket) : static_cast<int>(blockIdx.x);
-    const int place = id / p.slabs, slab = id - place * p.slabs;
-    const int tile = p.tiles - 1 - place;
-    const int first = tile * kTileRows;
-    const int segment = threadIdx.x / Q;
-    const int in_slab = (threadIdx.x % Q) * V;
-    const int c = slab * C + in_slab;
-    const bool in = c < p.channels;
-    const int begin = first + segment * kSegmentRows;
+// e_t = a_t dh_t is what a row hands to the row before it: e_t = a_t e_{t+1} + a_t dy_t, a chain
+// of the same kind backwards in time. A tile's map needs no walk backwards: what it hands out is
+// the sum of its dy_t times the product of its gates up to t, as far as the first sequence's end.
+template <typename T, bool Whole>
+__global__ void __launch_bounds__(kThreads, 3) recurrence_flow_maps_kernel(ScanArgs<T> p) {
+    constexpr int R = kRingRows, S = kRingStages;
+    const Walk<T, Whole, true> walk(p, blockIdx.x);
+    const Ring<T, Whole, 2, R, S> ring;
+    Row<T> prod = Row<T>::filled(1.0f), e = Row<T>::filled(0.0f);
+    bool open = true;
+    if (walk.count > 0) {
+        const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
+        const auto fetch = [&](int row, int stage) {
+            if (row < end) {
+                ring.fetch(walk, stage, 0, p.dy, p.dy_stride, p.order, row, end);
+                ring.fetch(walk, stage, 1, p.z, p.z_stride, p.order, row, end);
+            }
+            ring.commit();
+        };
+#pragma unroll
+        for (int s = 0; s < S - 1; ++s) {
+            fetch(first + s * R, s);
+        }
+        Cursor cursor;
+        cursor.seek(p.order, first);
+        open = first >= cursor.begin;   // a row outside all sequences hands nothing out
+        int stage = 0;
+#pragma unroll 1
+        for (int row = first; open && row < end; row += R) {
+            ring.wait();
+            fetch(row + (S - 1) * R, (stage + S - 1) % S);
+            const auto scan = [&](auto marked) {
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const bool ends = decltype(marked)::value && row + r == cursor.end - 1;
+                    const Row<T> a = gates<T>(ring.row(stage, 1, r));
+                    Row<T> up = ring.row(stage, 0, r);
+                    if (ends) {
+                        const Row<T> more = walk.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
+#pragma unroll
+                        for (int i = 0; i < Row<T>::kPairs; ++i) {
+                            up.v[i] = up.v[i] + more.v[i];
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < Row<T>::kPairs; ++i) {
+                        prod.v[i] = prod.v[i] * a.v[i];
+                        e.v[i] = fma(prod.v[i], up.v[i], e.v[i]);
+                    }
+                    if (ends) {
+                        open = false;
+                        break;
+                    }
+                }
+            };
+            if (cursor.covers(row, R)) {
+                scan(Flag<false>{});
+            } else {
+                scan(Flag<true>{});
+            }
+            stage = (stage + 1) % S;
+        }
+    }
+    share_maps<T>(p, walk, !open, prod, e);
+}
 
-    Pack<T, V> x[kSegmentRows], dy[kSegmentRows], z[kSegmentRows];
-#pragma unroll
-    for (int r = 0; r < kSegmentRows; ++r) {
-        const bool live = in && begin + r < p.order.rows;
-        const size_t row = live ? p.order.row(begin + r) : 0;
-        x[r] = live ? load_pack<T, V>(p.x + row * p.x_stride + c) : zero_pack<T, V>();
-        z[r] = live ? load_pack<T, V>(p.z + row * p.z_stride + c) : zero_pack<T, V>();
-        dy[r] = live ? load_pack<T, V>(p.dy + row * p.dy_stride + c) : zero_pack<T, V>();
-    }
-    fill_rows(table, p.order, first, p.chain.status);
-
-    float a[kSegmentRows][V], prod[V], h[V], e[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        prod[i] = 1.0f;
-        h[i] = e[i] = 0.0f;
-    }
-    bool cut = false, flow_cut = false;
-#pragma unroll
-    for (int r = 0; r < kSegmentRows; ++r) {
-        const int head = table.head[segment * kSegmentRows + r];
-        if (head != -1) {
-            cut = true;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                h[i] = head >= 0 && in && p.initial != nullptr
-                           ? p.initial[static_cast<size_t>(p.order.sequence(head)) * p.channels + c + i]
-                           : 0.0f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            a[r][i] = sigmoid_gate(z[r].get(i));
-            prod[i] *= a[r][i];
-            h[i] = fmaf(a[r][i], h[i], (1.0f - a[r][i]) * x[r].get(i));
-            if (head == -2) {
-                h[i] = 0.0f;
-            }
-        }
-    }
-#pragma unroll
-    for (int r = kSegmentRows - 1; r >= 0; --r) {
-        const int head = table.head[segment * kSegmentRows + r], tail = table.tail[segment * kSegmentRows + r];
-        if (tail >= 0 || head == -2) {
-            flow_cut = true;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                e[i] = tail >= 0 && in && p.dfinal != nullptr
-                           ? p.dfinal[static_cast<size_t>(p.order.sequence(tail)) * p.channels + c + i]
-                           : 0.0f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            e[i] = head == -2 ? 0.0f : a[r][i] * (dy[r].get(i) + e[i]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        maps[segment][in_slab + i] = make_float2(cut ? kReset : prod[i], h[i]);
-        flows[segment][in_slab + i] = make_float2(flow_cut ? kReset : prod[i], e[i]);
-    }
-    __syncthreads();
-    if (threadIdx.x < C) {
-        const int channel = slab * C + threadIdx.x;
-        float2 own = make_float2(1.0f, 0.0f);
-#pragma unroll
-        for (int s = kSegments - 1; s >= 0; --s) {
-            own = compose(own, flows[s][threadIdx.x]);
-        }
-        float flow = 0.0f;
-        if (channel < p.channels && p.tiles > 1) {
-            // the tile's last row decides whether what comes from behind matters
-            const bool open = table.tail[kTileRows - 1] < 0 && table.head[kTileRows - 1] != -2;
-            flow = chain_through(p.chain, place, p.tiles, p.channels, channel, own, open);
-        }
-        for (int s = kSegments - 1; s >= 0; --s) {
-            const float2 map = flows[s][threadIdx.x];
-            flows[s][threadIdx.x].y = flow;
-            flow = apply(map, flow);
-        }
-        float state = channel < p.channels ? p.carries[static_cast<size_t>(tile) * p.channels + channel] : 0.0f;
-        for (int s = 0; s < kSegments; ++s) {
-            const float2 map = maps[s][threadIdx.x];
-            maps[s][threadIdx.x].y = state;
-            state = apply(map, state);
-        }
-    }
-    __syncthreads();
-    if (!in) {
+// Batches of rows from the last to the first. With q_t = a_t (h_{t-1} - x_t): h_t = x_t + q_t,
+// and dz_t = dx_t q_t.
+template <typename T, bool Whole>
+__global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanArgs<T> p) {
+    constexpr int R = kCarryRows, P = Row<T>::kPairs;
+    const int block = gridDim.x - 1 - blockIdx.x;
+    const Walk<T, Whole, true> walk(p, block);
+    const Ring<T, Whole, 3, R, 2> ring;
+    if (walk.count == 0) {
         return;
     }
-    float before[kSegmentRows][V];
+    const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
+    const auto fetch = [&](int row, int stage) {
+        if (row >= first) {
+            ring.fetch(walk, stage, 0, p.x, p.x_stride, p.order, row, end);
+            ring.fetch(walk, stage, 1, p.z, p.z_stride, p.order, row, end);
+            ring.fetch(walk, stage, 2, p.dy, p.dy_stride, p.order, row, end);
+        }
+        ring.commit();
+    };
+    const int last = first + (end - 1 - first) / R * R;
+    fetch(last, 0);
+    Row<T> e = reaching_state<T>(p, walk, block);
+    const long long down = walk.row_step * p.channels;
+    int stage = 0;
+#pragma unroll 1
+    for (int row = last; row >= first; row -= R) {
+        Row<T> h = walk.state(p.carries, row / R, p.channels);
+        Cursor cursor;
+        cursor.seek(p.order, row);
+        const bool covered = cursor.covers(row, R);
+        // of the batch's rows: start a sequence, end one, lie outside all
+        unsigned heads = 0, tails = 0, dead = 0;
+        if (!covered) {
+            Cursor at = cursor;
+            for (int r = 0; r < R; ++r) {
+                dead |= row + r < at.begin ? 1u << r : 0u;
+                heads |= row + r == at.begin ? 1u << r : 0u;
+                if (row + r == at.end - 1) {
+                    tails |= 1u << r;
+                    at.next(p.order);
+                }
+            }
+        }
+        ring.wait();
+        fetch(row - R, stage ^ 1);
+        const long long at0 = static_cast<long long>(p.order.row(row)) * p.channels + walk.c;
+        const auto differentiate = [&](auto marked) {
+            Row<T> odds[R], q[R];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        h[i] = maps[segment][in_slab + i].y;
-        e[i] = flows[segment][in_slab + i].y;
+            for (int r = 0; r < R; ++r) {
+                if (decltype(marked)::value && (heads >> r & 1u)) {
+                    h = walk.state(p.initial, p.order.sequence(cursor.j), p.channels);
+                }
+                const Row<T> zr = ring.row(stage, 1, r), xr = ring.row(stage, 0, r);
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    odds[r].v[i] = exp_minus({max_or_nan(zr.v[i].x, kLowestGate), max_or_nan(zr.v[i].y, kLowestGate)});
+                    q[r].v[i] = sigmoid_from(odds[r].v[i]) * minus(h.v[i], xr.v[i]);
+                    h.v[i] = xr.v[i] + q[r].v[i];
+                }
+                if (decltype(marked)::value && (tails >> r & 1u)) {
+                    cursor.next(p.order);
+                }
+            }
+#pragma unroll
+            for (int r = R - 1; r >= 0; --r) {
+                if (decltype(marked)::value && (tails >> r & 1u)) {
+                    cursor.seek(p.order, row + r);
+                    e = walk.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
+                }
+                const Row<T> up = ring.row(stage, 2, r);
+                Row<T> dx, dz;
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    e.v[i] = sigmoid_from(odds[r].v[i]) * (up.v[i] + e.v[i]);
+                    dx.v[i] = odds[r].v[i] * e.v[i];   // exp(-z) sigmoid(z) dh = sigmoid(-z) dh
+                    dz.v[i] = dx.v[i] * q[r].v[i];
+                }
+                if (decltype(marked)::value && (dead >> r & 1u)) {
+                    dx = dz = e = Row<T>::filled(0.0f);
+                }
+                if (!decltype(marked)::value || row + r < end) {
+                    walk.store(p.dx + at0 + r * down, dx);
+                    walk.store(p.dz + at0 + r * down, dz);
+                }
+                if (decltype(marked)::value && (heads >> r & 1u)) {
+                    cursor.seek(p.order, row + r);
+                    walk.store_state(p.dinitial, p.order.sequence(cursor.j), p.channels, e);
+                }
+            }
+        };
+        if (covered) {
+            differentiate(Flag<false>{});
+        } else {
+            differentiate(Flag<true>{});
+        }
+        stage ^= 1;
     }
-#pragma unroll
-    for (int r = 0; r < kSegmentRows; ++r) {
-        const int head = table.head[segment * kSegmentRows + r];
-        if (head >= 0) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                h[i] = p.initial != nullptr
-                           ? p.initial[static_cast<size_t>(p.order.sequence(head)) * p.channels + c + i]
-                           : 0.0f;
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            before[r][i] = h[i];
-            h[i] = fmaf(a[r][i], h[i], (1.0f - a[r][i]) * x[r].get(i));
+}
+
+// From the groups' maps to the state that reaches each group: kScanChannels channels a block,
+// kScanParts threads a channel. A thread composes a run of groups, the threads of a channel scan
+// their maps, and each walks its run again.
+constexpr int kScanChannels = 8, kScanParts = 128;
+
+__global__ void __launch_bounds__(kScanChannels * kScanParts) recurrence_scan_kernel(
+    const float2* groups, int count, int channels, float* states
+) {
+    __shared__ float2 maps[kScanParts][kScanChannels];
+    const int lane = threadIdx.x % kScanChannels, part = threadIdx.x / kScanChannels;
+    const int c = blockIdx.x * kScanChannels + lane;
+    const bool in = c < channels;
+    const int run = (count + kScanParts - 1) / kScanParts;
+    const int begin = min(part * run, count), end = min(begin + run, count);
+    float2 map = make_float2(1.0f, 0.0f);
+    if (in) {
+#pragma unroll 4
+        for (int g = begin; g < end; ++g) {
+            map = compose(map, groups[static_cast<size_t>(g) * channels + c]);
         }
     }
-#pragma unroll
-    for (int r = kSegmentRows - 1; r >= 0; --r) {
-        if (begin + r >= p.order.rows) {
-            continue;
-        }
-        const int head = table.head[segment * kSegmentRows + r], tail = table.tail[segment * kSegmentRows + r];
-        if (tail >= 0) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                e[i] = p.dfinal != nullptr
-                           ? p.dfinal[static_cast<size_t>(p.order.sequence(tail)) * p.channels + c + i]
-                           : 0.0f;
-            }
-        }
-        Pack<T, V> dx, dz;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float gate, rest;
-            sigmoid_pair(z[r].get(i), gate, rest);
-            const float dh = dy[r].get(i) + e[i];
-            const float dxi = rest * dh;
-            dx.set(i, head == -2 ? 0.0f : dxi);
-            dz.set(i, head == -2 ? 0.0f : a[r][i] * dxi * (before[r][i] - x[r].get(i)));
-            e[i] = head == -2 ? 0.0f : a[r][i] * dh;
-        }
-        const size_t row = p.order.row(begin + r);
-        store_pack<T, V>(p.dx + row * p.channels + c, dx);
-        store_pack<T, V>(p.dz + row * p.channels + c, dz);
-        if (head >= 0 && p.dinitial != nullptr) {
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                p.dinitial[static_cast<size_t>(p.order.sequence(head)) * p.channels + c + i] = e[i];
-            }
+    maps[part][lane] = map;
+    __syncthreads();
+    for (int d = 1; d < kScanParts; d <<= 1) {
+        const float2 before = part >= d ? maps[part - d][lane] : make_float2(1.0f, 0.0f);
+        __syncthreads();
+        map = compose(before, map);
+        maps[part][lane] = map;
+        __syncthreads();
+    }
+    float h = part > 0 ? apply(maps[part - 1][lane], 0.0f) : 0.0f;
+    if (in) {
+#pragma unroll 4
+        for (int g = begin; g < end; ++g) {
+            states[static_cast<size_t>(g) * channels + c] = h;
+            h = apply(groups[static_cast<size_t>(g) * channels + c], h);
         }
     }
 }
@@ -586,89 +814,99 @@ constexpr int kMaxRows = 0x7fffffff - kTileRows;   // row numbers of the last ti
 
 inline int tiles_of(long long rows) { return static_cast<int>((rows + kTileRows - 1) / kTileRows); }
 
-struct ChainBytes {
-    size_t tiles, groups, states, total;
-};
-
-inline ChainBytes chain_bytes(long long rows, int channels) {
-    ChainBytes b{};
-    const long long tiles = tiles_of(rows);
-    const long long groups = (tiles + kGroup - 1) / kGroup;
-    const size_t line = sizeof(unsigned long long) * channels;
-    b.tiles = align_up(line * tiles);
-    b.groups = align_up(line * groups);
-    b.states = align_up(line * ((groups + kGroup - 1) / kGroup + 1));
-    b.total = 256 + b.tiles + b.groups + b.states;
-    return b;
-}
-
-template <typename T> int prepare_chain(ScanArgs<T>& p, void* workspace, size_t bytes, int32_t* status, cudaStream_t stream) {
-    p.tiles = tiles_of(p.order.rows);
-    p.chain.budget = wait_budget_cycles();
-    p.chain.status = status;
-    if (p.tiles <= 1) {
-        return LAT_OK;
-    }
-    const ChainBytes b = chain_bytes(p.order.rows, p.channels);
-    if (workspace == nullptr || bytes < b.total) {
-        return fail(LAT_WORKSPACE_TOO_SMALL, "recurrence workspace is too small.");
-    }
-    char* base = static_cast<char*>(workspace);
-    p.chain.ticket = reinterpret_cast<int*>(base);
-    p.chain.tiles = reinterpret_cast<unsigned long long*>(base + 256);
-    p.chain.groups = reinterpret_cast<unsigned long long*>(base + 256 + b.tiles);
-    p.chain.states = reinterpret_cast<unsigned long long*>(base + 256 + b.tiles + b.groups);
-    // all ones: unwritten records, and a ticket of -1
-    LAT_CUDA_CHECK(cudaMemsetAsync(workspace, 0xFF, b.total, stream));
-    return LAT_OK;
-}
-
-// Threads across a slab: eight vectors (a 128-byte line of the forward pass), fewer where the
-// row is shorter or a smaller slab leaves fewer idle threads.
-inline int slab_threads(int vectors) {
-    int best = 8;
-    for (int q = 8; q >= 1; q >>= 1) {
-        const int slots = (vectors + q - 1) / q * q, best_slots = (vectors + best - 1) / best * best;
-        if (slots < best_slots) {
-            best = q;
+// Threads across a slab for `vectors` of eight bytes: 16, a 128-byte line, or fewer where that
+// leaves fewer of them without a channel.
+inline int slab_lanes(int vectors) {
+    int best = 16;
+    for (int lanes = 16; lanes >= 1; lanes >>= 1) {
+        if ((vectors + lanes - 1) / lanes * lanes < (vectors + best - 1) / best * best) {
+            best = lanes;
         }
     }
     return best;
 }
 
-template <typename T, int V, int Q, bool Backward> int launch_scan(ScanArgs<T> p, cudaStream_t stream) {
-    p.slabs = (p.channels + V * Q - 1) / (V * Q);
-    const long long blocks = static_cast<long long>(p.tiles) * p.slabs;
-    LAT_REQUIRE(blocks <= 0x7fffffffLL, "the recurrence supports at most 2^31 tiles.");
+struct ScanBytes {
+    size_t maps, groups, states, total;
+};
+
+inline ScanBytes scan_bytes(long long rows, int channels, int wide) {
+    ScanBytes b{};
+    const long long tiles = tiles_of(rows), per_group = kThreads / slab_lanes((channels + wide - 1) / wide);
+    const long long groups = (tiles + per_group - 1) / per_group;
+    b.maps = align_up(sizeof(float2) * channels * tiles);
+    b.groups = align_up(sizeof(float2) * channels * groups);
+    b.states = align_up(sizeof(float) * channels * groups);
+    b.total = tiles <= 1 ? 256 : b.maps + b.groups + b.states;
+    return b;
+}
+
+template <typename T, bool Whole, bool Backward>
+int launch_scan(ScanArgs<T> p, void* workspace, size_t bytes, cudaStream_t stream) {
+    p.tiles = tiles_of(p.order.rows);
+    const int vectors = (p.channels + kWide<T> - 1) / kWide<T>;
+    p.lanes = slab_lanes(vectors);
+    p.slabs = (vectors + p.lanes - 1) / p.lanes;
+    const int per_group = kThreads / p.lanes;
+    const int groups = (p.tiles + per_group - 1) / per_group;
+    const long long blocks = static_cast<long long>(groups) * p.slabs;
+    LAT_REQUIRE(blocks <= 0x7fffffffLL, "the recurrence supports at most 2^31 blocks of tiles.");
+    const ScanBytes b = scan_bytes(p.order.rows, p.channels, kWide<T>);
+    if (workspace == nullptr || bytes < b.total) {
+        return fail(LAT_WORKSPACE_TOO_SMALL, "recurrence workspace is too small.");
+    }
+    const unsigned grid = static_cast<unsigned>(blocks);
+    constexpr int kRing = Ring<T, Whole, 2, kRingRows, kRingStages>::kBytes;
+    constexpr int kApplyRing = Backward ? Ring<T, Whole, 3, kCarryRows, 2>::kBytes : kRing;
+    const void *maps_kernel, *apply_kernel;
     if constexpr (Backward) {
-        recurrence_backward_kernel<T, V, Q><<<static_cast<unsigned>(blocks), Q * kSegments, 0, stream>>>(p);
+        maps_kernel = reinterpret_cast<const void*>(recurrence_flow_maps_kernel<T, Whole>);
+        apply_kernel = reinterpret_cast<const void*>(recurrence_gradient_kernel<T, Whole>);
     } else {
-        recurrence_forward_kernel<T, V, Q><<<static_cast<unsigned>(blocks), Q * kSegments, 0, stream>>>(p);
+        maps_kernel = reinterpret_cast<const void*>(recurrence_maps_kernel<T, Whole>);
+        apply_kernel = reinterpret_cast<const void*>(recurrence_apply_kernel<T, Whole>);
+    }
+    LAT_CUDA_CHECK(cudaFuncSetAttribute(maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
+    LAT_CUDA_CHECK(cudaFuncSetAttribute(apply_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kApplyRing));
+    if (p.tiles > 1) {
+        char* base = static_cast<char*>(workspace);
+        p.maps = reinterpret_cast<float2*>(base);
+        p.groups = reinterpret_cast<float2*>(base + b.maps);
+        if constexpr (Backward) {
+            recurrence_flow_maps_kernel<T, Whole><<<grid, kThreads, kRing, stream>>>(p);
+        } else {
+            recurrence_maps_kernel<T, Whole><<<grid, kThreads, kRing, stream>>>(p);
+        }
+        LAT_LAUNCH_CHECK();
+        if (groups > 1) {
+            p.states = reinterpret_cast<float*>(base + b.maps + b.groups);
+            recurrence_scan_kernel<<<(p.channels + kScanChannels - 1) / kScanChannels, kScanChannels * kScanParts, 0,
+                                     stream>>>(p.groups, groups, p.channels, p.states);
+            LAT_LAUNCH_CHECK();
+        }
+    }
+    if constexpr (Backward) {
+        recurrence_gradient_kernel<T, Whole><<<grid, kThreads, kApplyRing, stream>>>(p);
+    } else {
+        recurrence_apply_kernel<T, Whole><<<grid, kThreads, kApplyRing, stream>>>(p);
     }
     LAT_LAUNCH_CHECK();
     return LAT_OK;
 }
 
-template <typename T, bool Backward> int run_scan(const ScanArgs<T>& p, cudaStream_t stream) {
-    constexpr int V = 16 / sizeof(T);
-    bool vec = p.channels % V == 0 && p.x_stride % V == 0 && p.z_stride % V == 0 && aligned_to(p.x, 16) &&
-               aligned_to(p.z, 16);
+template <typename T, bool Backward>
+int run_scan(const ScanArgs<T>& p, void* workspace, size_t bytes, cudaStream_t stream) {
+    constexpr int N = kWide<T>;
+    bool whole = p.channels % N == 0 && p.x_stride % N == 0 && p.z_stride % N == 0 && aligned_to(p.x, 8) && aligned_to(p.z, 8) &&
+                 aligned_to(p.carries, sizeof(float) * N) && aligned_to(p.initial, sizeof(float) * N);
     if (Backward) {
-        vec = vec && p.dy_stride % V == 0 && aligned_to(p.dy, 16) && aligned_to(p.dx, 16) && aligned_to(p.dz, 16);
+        whole = whole && p.dy_stride % N == 0 && aligned_to(p.dy, 8) && aligned_to(p.dx, 8) && aligned_to(p.dz, 8) &&
+                aligned_to(p.dinitial, sizeof(float) * N) && aligned_to(p.dfinal, sizeof(float) * N);
     } else {
-        vec = vec && aligned_to(p.h, 16);
+        whole = whole && aligned_to(p.h, 8) && aligned_to(p.final, sizeof(float) * N);
     }
-    if (!vec) {
-        return launch_scan<T, 1, 32, Backward>(p, stream);
-    }
-    // the backward pass holds twice as many values per element: half as many channels a thread
-    constexpr int W = Backward ? V / 2 : V, M = V / W;
-    switch (slab_threads(p.channels / V)) {
-        case 8: return launch_scan<T, W, 8 * M, Backward>(p, stream);
-        case 4: return launch_scan<T, W, 4 * M, Backward>(p, stream);
-        case 2: return launch_scan<T, W, 2 * M, Backward>(p, stream);
-        default: return launch_scan<T, W, M, Backward>(p, stream);
-    }
+    return whole ? launch_scan<T, true, Backward>(p, workspace, bytes, stream)
+                 : launch_scan<T, false, Backward>(p, workspace, bytes, stream);
 }
 
 // What a sequence without rows hands on: initial -> final, dfinal -> dinitial.
@@ -700,8 +938,8 @@ int forward_typed(const void* x, long long x_stride, const void* z, long long z_
     p.carries = carries;
     p.h = static_cast<T*>(h);
     p.final = final;
-    const int code = prepare_chain(p, workspace, bytes, status, stream);
-    return code != LAT_OK ? code : run_scan<T, false>(p, stream);
+    p.status = status;
+    return run_scan<T, false>(p, workspace, bytes, stream);
 }
 
 template <typename T>
@@ -724,8 +962,8 @@ int backward_typed(const void* dy, long long dy_stride, const float* dfinal, con
     p.dx = static_cast<T*>(dx);
     p.dz = static_cast<T*>(dz);
     p.dinitial = dinitial;
-    const int code = prepare_chain(p, workspace, bytes, status, stream);
-    return code != LAT_OK ? code : run_scan<T, true>(p, stream);
+    p.status = status;
+    return run_scan<T, true>(p, workspace, bytes, stream);
 }
 
 } // namespace
@@ -736,14 +974,16 @@ using namespace lat;
 
 extern "C" {
 
-size_t lat_recurrence_workspace_bytes(int32_t rows, int32_t channels) {
-    if (rows <= kTileRows || channels <= 0) {
+size_t lat_recurrence_workspace_bytes(int32_t dtype, int32_t rows, int32_t channels) {
+    if (rows <= 0 || channels <= 0) {
         return 256;
     }
-    return chain_bytes(rows, channels).total;
+    return scan_bytes(rows, channels, dtype == LAT_F32 ? kWide<float> : kWide<__half>).total;
 }
 
-int32_t lat_recurrence_tiles(int32_t rows) { return rows <= 0 ? 0 : tiles_of(rows); }
+int32_t lat_recurrence_carry_rows(int32_t rows) {
+    return rows <= 0 ? 0 : (rows - 1) / kCarryRows + 1;
+}
 
 int lat_recurrence_forward(
     int32_t dtype, const void* feats, int64_t feat_row_stride, const void* gate, int64_t gate_row_stride,

@@ -51,73 +51,101 @@ template <typename T> struct NormArgs {
     float* partial;   // [gridDim.x][2][channels]
 };
 
+// Rows that a group of lanes has in flight: with K vectors a lane, enough of them that a
+// thread waits for about 64 bytes of x at once (the memory needs some 50 KB in flight per SM).
+template <int K> constexpr int kRowsInFlight = K == 1 ? 4 : K <= 3 ? 2 : 1;
+
 // A lane owns the vectors lane, lane + L, ... of its row: K vectors of V elements.
 template <typename T, int V, int K, bool Rms>
 __global__ void __launch_bounds__(kThreads) norm_forward_kernel(NormArgs<T> p) {
+    constexpr int U = kRowsInFlight<K>;
     const int lane = threadIdx.x & 31;
     const int sub = lane & (p.lanes - 1);
     const int rows_per_warp = 32 / p.lanes;
-    const float inv_c = static_cast<float>(p.channels);
-    const long long warps = static_cast<long long>(gridDim.x) * kWarps;
+    const float count = static_cast<float>(p.channels);
     const long long warp = blockIdx.x * static_cast<long long>(kWarps) + (threadIdx.x >> 5);
-    for (long long row0 = warp * rows_per_warp; row0 < p.rows; row0 += warps * rows_per_warp) {
-        const long long row = row0 + lane / p.lanes;
-        const bool live = row < p.rows;
-        Pack<T, V> x[K];
-        float sum = 0.0f;
+    const long long row0 = warp * rows_per_warp * U + lane / p.lanes;
+    Pack<T, V> x[U][K];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const long long row = row0 + u * rows_per_warp;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             const int c = (sub + k * p.lanes) * V;
-            x[k] = live && c < p.channels ? load_pack<T, V>(p.x + row * p.x_stride + c) : zero_pack<T, V>();
+            x[u][k] = row < p.rows && c < p.channels ? load_pack<T, V>(p.x + row * p.x_stride + c) : zero_pack<T, V>();
+        }
+    }
+    float mean[U], r[U];
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                sum += x[k].get(i);
+    for (int u = 0; u < U; ++u) {
+        float sum = 0.0f;
+        if (!Rms) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    sum += x[u][k].get(i);
+                }
             }
         }
-        const float mean = Rms ? 0.0f : group_sum(sum, p.lanes) / inv_c;
+        mean[u] = Rms ? 0.0f : group_sum(sum, p.lanes) / count;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
         float squares = 0.0f;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if ((sub + k * p.lanes) * V < p.channels) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float d = x[k].get(i) - mean;
+                    const float d = x[u][k].get(i) - mean[u];
                     squares = fmaf(d, d, squares);
                 }
             }
         }
-        const float r = rsqrtf(group_sum(squares, p.lanes) / inv_c + p.eps);
-        if (!live) {
-            continue;
-        }
-        if (sub == 0) {
-            p.rstd[row] = r;
-            if (!Rms) {
-                p.mean[row] = mean;
+        r[u] = rsqrtf(group_sum(squares, p.lanes) / count + p.eps);
+    }
+    if (sub == 0) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long row = row0 + u * rows_per_warp;
+            if (row < p.rows) {
+                p.rstd[row] = r[u];
+                if (!Rms) {
+                    p.mean[row] = mean[u];
+                }
             }
         }
+    }
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (sub + k * p.lanes) * V;
-            if (c < p.channels) {
-                Pack<T, V> w, b, y;
+    for (int k = 0; k < K; ++k) {
+        const int c = (sub + k * p.lanes) * V;
+        if (c >= p.channels) {
+            break;
+        }
+        Pack<T, V> w, b;
+        if (p.weight != nullptr) {
+            w = load_pack<T, V>(p.weight + c);
+        }
+        if (p.bias != nullptr) {
+            b = load_pack<T, V>(p.bias + c);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const long long row = row0 + u * rows_per_warp;
+            Pack<T, V> y;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                float v = (x[u][k].get(i) - mean[u]) * r[u];
                 if (p.weight != nullptr) {
-                    w = load_pack<T, V>(p.weight + c);
+                    v *= w.get(i);
                 }
                 if (p.bias != nullptr) {
-                    b = load_pack<T, V>(p.bias + c);
+                    v += b.get(i);
                 }
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float v = (x[k].get(i) - mean) * r;
-                    if (p.weight != nullptr) {
-                        v *= w.get(i);
-                    }
-                    if (p.bias != nullptr) {
-                        v += b.get(i);
-                    }
-                    y.set(i, v);
-                }
+                y.set(i, v);
+            }
+            if (row < p.rows) {
                 store_pack<T, V>(p.out + row * p.channels + c, y);
             }
         }
@@ -125,83 +153,88 @@ __global__ void __launch_bounds__(kThreads) norm_forward_kernel(NormArgs<T> p) {
 }
 
 template <typename T, int V, int K, bool Rms>
-__global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p) {
-    extern __shared__ float sums[];  // [2][channels]
+__global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p, T* dw_out, T* db_out) {
+    constexpr int U = kRowsInFlight<K>;
+    extern __shared__ float sums[];  // [kWarps / 2][2][channels]
     const int lane = threadIdx.x & 31;
     const int sub = lane & (p.lanes - 1);
     const int rows_per_warp = 32 / p.lanes;
     const float count = static_cast<float>(p.channels);
-    const long long warps = static_cast<long long>(gridDim.x) * kWarps;
-    const long long warp = blockIdx.x * static_cast<long long>(kWarps) + (threadIdx.x >> 5);
+    const long long step = static_cast<long long>(gridDim.x) * kWarps * rows_per_warp * U;
+    const int warp = threadIdx.x >> 5;
     float dw[K][V], db[K][V];
+    Pack<T, V> w[K];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
+        const int c = (sub + k * p.lanes) * V;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             dw[k][i] = db[k][i] = 0.0f;
+            w[k].set(i, 1.0f);
+        }
+        if (p.weight != nullptr && c < p.channels) {
+            w[k] = load_pack<T, V>(p.weight + c);
         }
     }
-    for (long long row0 = warp * rows_per_warp; row0 < p.rows; row0 += warps * rows_per_warp) {
-        const long long row = row0 + lane / p.lanes;
-        const bool live = row < p.rows;
-        Pack<T, V> x[K], dy[K];
+    for (long long base = (blockIdx.x * static_cast<long long>(kWarps) + warp) * rows_per_warp * U; base < p.rows;
+         base += step) {
+        const long long row0 = base + lane / p.lanes;
+        Pack<T, V> x[U][K], dy[U][K];
+        float r[U], mean[U];
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (sub + k * p.lanes) * V;
-            const bool in = live && c < p.channels;
-            x[k] = in ? load_pack<T, V>(p.x + row * p.x_stride + c) : zero_pack<T, V>();
-            dy[k] = in ? load_pack<T, V>(p.dy + row * p.dy_stride + c) : zero_pack<T, V>();
+        for (int u = 0; u < U; ++u) {
+            const long long row = row0 + u * rows_per_warp;
+            const bool live = row < p.rows;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const int c = (sub + k * p.lanes) * V;
+                const bool in = live && c < p.channels;
+                x[u][k] = in ? load_pack<T, V>(p.x + row * p.x_stride + c) : zero_pack<T, V>();
+                dy[u][k] = in ? load_pack<T, V>(p.dy + row * p.dy_stride + c) : zero_pack<T, V>();
+            }
+            r[u] = live ? p.rstd[row] : 0.0f;
+            mean[u] = !Rms && live ? p.mean[row] : 0.0f;
         }
-        const float r = live ? p.rstd[row] : 0.0f;
-        const float mean = !Rms && live ? p.mean[row] : 0.0f;
-        float c1 = 0.0f, c2 = 0.0f;
 #pragma unroll
-        for (int k = 0; k < K; ++k) {
-            const int c = (sub + k * p.lanes) * V;
-            if (c < p.channels) {
-                Pack<T, V> w;
-                if (p.weight != nullptr) {
-                    w = load_pack<T, V>(p.weight + c);
-                }
+        for (int u = 0; u < U; ++u) {
+            const long long row = row0 + u * rows_per_warp;
+            float c1 = 0.0f, c2 = 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const float d = dy[k].get(i);
-                    const float xh = (x[k].get(i) - mean) * r;
-                    const float g = p.weight != nullptr ? d * w.get(i) : d;
+                    // zeros beyond the row's end: dy and with it every term is zero there
+                    const float d = dy[u][k].get(i);
+                    const float xh = (x[u][k].get(i) - mean[u]) * r[u];
+                    const float g = d * w[k].get(i);
                     c1 += g;
                     c2 = fmaf(g, xh, c2);
                     dw[k][i] = fmaf(d, xh, dw[k][i]);
                     db[k][i] += d;
                 }
             }
-        }
-        c1 = Rms ? 0.0f : group_sum(c1, p.lanes) / count;
-        c2 = group_sum(c2, p.lanes) / count;
-        if (live) {
+            c1 = Rms ? 0.0f : group_sum(c1, p.lanes) / count;
+            c2 = group_sum(c2, p.lanes) / count;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int c = (sub + k * p.lanes) * V;
-                if (c < p.channels) {
-                    Pack<T, V> w, dx;
-                    if (p.weight != nullptr) {
-                        w = load_pack<T, V>(p.weight + c);
-                    }
+                Pack<T, V> dx;
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        const float d = dy[k].get(i);
-                        const float xh = (x[k].get(i) - mean) * r;
-                        const float g = p.weight != nullptr ? d * w.get(i) : d;
-                        dx.set(i, r * (g - c1 - xh * c2));
-                    }
+                for (int i = 0; i < V; ++i) {
+                    const float xh = (x[u][k].get(i) - mean[u]) * r[u];
+                    dx.set(i, r[u] * (dy[u][k].get(i) * w[k].get(i) - c1 - xh * c2));
+                }
+                if (row < p.rows && c < p.channels) {
                     store_pack<T, V>(p.out + row * p.channels + c, dx);
                 }
             }
         }
     }
-    if (p.partial == nullptr) {
+    if (dw_out == nullptr && db_out == nullptr) {
         return;
     }
-    // lanes of the warp that own the same channels, then the warps one after the other
+    // lanes of the warp that own the same channels; the upper warps' sums to the lower ones;
+    // then the four sums of each channel
     for (int d = p.lanes; d < 32; d <<= 1) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
@@ -212,16 +245,19 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p) 
             }
         }
     }
-    for (int w = 0; w < kWarps; ++w) {
-        if ((threadIdx.x >> 5) == w && lane < p.lanes) {
+    constexpr int kHalf = kWarps / 2;
+    float* mine = sums + static_cast<size_t>(warp % kHalf) * 2 * p.channels;
+#pragma unroll
+    for (int phase = 0; phase < 2; ++phase) {
+        if ((warp >= kHalf) == (phase == 0) && lane < p.lanes) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 const int c = (sub + k * p.lanes) * V;
                 if (c < p.channels) {
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        sums[c + i] = (w == 0 ? 0.0f : sums[c + i]) + dw[k][i];
-                        sums[p.channels + c + i] = (w == 0 ? 0.0f : sums[p.channels + c + i]) + db[k][i];
+                        mine[c + i] = phase == 0 ? dw[k][i] : dw[k][i] + mine[c + i];
+                        mine[p.channels + c + i] = phase == 0 ? db[k][i] : db[k][i] + mine[p.channels + c + i];
                     }
                 }
             }
@@ -230,7 +266,16 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p) 
     }
     float* partial = p.partial + static_cast<size_t>(blockIdx.x) * 2 * p.channels;
     for (int c = threadIdx.x; c < 2 * p.channels; c += kThreads) {
-        partial[c] = sums[c];
+        float total = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kHalf; ++q) {
+            total += sums[static_cast<size_t>(q) * 2 * p.channels + c];
+        }
+        if (gridDim.x > 1) {
+            partial[c] = total;
+        } else if (c < p.channels ? dw_out != nullptr : db_out != nullptr) {
+            (c < p.channels ? dw_out : db_out)[c < p.channels ? c : c - p.channels] = narrow<T>(total);
+        }
     }
 }
 
@@ -337,19 +382,22 @@ __global__ void __launch_bounds__(kThreads) norm_sums_wide_kernel(NormArgs<T> p,
     partial[p.channels + c] = db;
 }
 
-// Sum of the partial rows, 32 channels a block: eight threads of a channel walk every eighth
-// partial row, then their sums are added in order.
+// Sum of the partial rows, 32 channels a block: 32 threads of a channel walk every 32nd partial
+// row, then their sums are added in order.
+constexpr int kReduceParts = 32;
+
 template <typename T>
-__global__ void __launch_bounds__(kThreads) norm_reduce_kernel(
+__global__ void __launch_bounds__(32 * kReduceParts) norm_reduce_kernel(
     const float* partial, int blocks, int channels, T* dw, T* db
 ) {
-    __shared__ float tile[kWarps][33];
+    __shared__ float tile[kReduceParts][33];
     const int lane = threadIdx.x & 31;
     const int part = threadIdx.x >> 5;
     const int at = blockIdx.x * 32 + lane;  // over [2][channels]
     float sum = 0.0f;
     if (at < 2 * channels) {
-        for (int b = part; b < blocks; b += kWarps) {
+#pragma unroll 8
+        for (int b = part; b < blocks; b += kReduceParts) {
             sum += partial[static_cast<size_t>(b) * 2 * channels + at];
         }
     }
@@ -357,8 +405,9 @@ __global__ void __launch_bounds__(kThreads) norm_reduce_kernel(
     __syncthreads();
     if (part == 0 && at < 2 * channels) {
         float total = 0.0f;
-        for (int w = 0; w < kWarps; ++w) {
-            total += tile[w][lane];
+#pragma unroll
+        for (int q = 0; q < kReduceParts; ++q) {
+            total += tile[q][lane];
         }
         T* out = at < channels ? dw : db;
         if (out != nullptr) {
@@ -390,14 +439,16 @@ inline void split_row(int vectors, int max_per_lane, int& lanes, int& per_lane) 
     }
 }
 
-inline int norm_grid(long long rows, int lanes) {
-    const long long per_block = static_cast<long long>(kWarps) * (32 / lanes);
-    return static_cast<int>(std::max(1LL, std::min((rows + per_block - 1) / per_block, 148LL * 4)));
+inline long long blocks_of(long long rows, int lanes, int in_flight) {
+    const long long per_block = static_cast<long long>(kWarps) * (32 / lanes) * in_flight;
+    return (rows + per_block - 1) / per_block;
 }
 
 template <typename T, int V, int K>
 int launch_forward(const NormArgs<T>& p, bool rms, cudaStream_t stream) {
-    const int grid = norm_grid(p.rows, p.lanes);
+    const long long blocks = blocks_of(p.rows, p.lanes, kRowsInFlight<K>);
+    LAT_REQUIRE(blocks <= 0x7fffffffLL, "normalisation supports at most 2^31 blocks of rows.");
+    const unsigned grid = static_cast<unsigned>(blocks);
     if (rms) {
         norm_forward_kernel<T, V, K, true><<<grid, kThreads, 0, stream>>>(p);
     } else {
@@ -407,32 +458,41 @@ int launch_forward(const NormArgs<T>& p, bool rms, cudaStream_t stream) {
     return LAT_OK;
 }
 
-template <typename T, int V, int K>
-int launch_backward(const NormArgs<T>& p, bool rms, int grid, cudaStream_t stream) {
-    const size_t smem = sizeof(float) * 2 * p.channels;
-    if (rms) {
-        norm_backward_kernel<T, V, K, true><<<grid, kThreads, smem, stream>>>(p);
-    } else {
-        norm_backward_kernel<T, V, K, false><<<grid, kThreads, smem, stream>>>(p);
-    }
+constexpr int kMaxBackwardBlocks = 148 * 2;
+
+template <typename T> int launch_reduce(const NormArgs<T>& p, int blocks, T* dw, T* db, cudaStream_t stream) {
+    norm_reduce_kernel<T><<<(2 * p.channels + 31) / 32, 32 * kReduceParts, 0, stream>>>(
+        p.partial, blocks, p.channels, dw, db);
     LAT_LAUNCH_CHECK();
     return LAT_OK;
 }
 
-// grid 0: forward
-template <typename T, int V>
-int dispatch_split(NormArgs<T> p, bool rms, int grid, cudaStream_t stream) {
+template <typename T, int V, int K>
+int launch_backward(const NormArgs<T>& p, bool rms, T* dw, T* db, cudaStream_t stream) {
+    const size_t smem = sizeof(float) * kWarps * p.channels;
+    const int grid = static_cast<int>(std::min<long long>(blocks_of(p.rows, p.lanes, kRowsInFlight<K>), kMaxBackwardBlocks));
+    if (rms) {
+        norm_backward_kernel<T, V, K, true><<<grid, kThreads, smem, stream>>>(p, dw, db);
+    } else {
+        norm_backward_kernel<T, V, K, false><<<grid, kThreads, smem, stream>>>(p, dw, db);
+    }
+    LAT_LAUNCH_CHECK();
+    return grid > 1 && (dw != nullptr || db != nullptr) ? launch_reduce(p, grid, dw, db, stream) : LAT_OK;
+}
+
+template <typename T, int V, bool Backward>
+int dispatch_split(NormArgs<T> p, bool rms, T* dw, T* db, cudaStream_t stream) {
     constexpr int kMost = kMaxLaneElements / V;
     int k;
     split_row(p.channels / V, kMost, p.lanes, k);
-    if (grid > 0) {
-        grid = std::min(grid, norm_grid(p.rows, p.lanes));
-    }
 #define LAT_NORM_CASE(N)                                                            \
     if constexpr (N <= kMost) {                                                     \
         if (k <= N) {                                                               \
-            return grid > 0 ? launch_backward<T, V, N>(p, rms, grid, stream)        \
-                            : launch_forward<T, V, N>(p, rms, stream);              \
+            if constexpr (Backward) {                                               \
+                return launch_backward<T, V, N>(p, rms, dw, db, stream);            \
+            } else {                                                                \
+                return launch_forward<T, V, N>(p, rms, stream);                     \
+            }                                                                       \
         }                                                                           \
     }
     LAT_NORM_CASE(1)
@@ -464,58 +524,42 @@ template <typename T> int run_forward(const NormArgs<T>& p, bool rms, cudaStream
         LAT_LAUNCH_CHECK();
         return LAT_OK;
     }
-    return vector_rows(p) ? dispatch_split<T, 16 / sizeof(T)>(p, rms, 0, stream)
-                          : dispatch_split<T, 1>(p, rms, 0, stream);
+    return vector_rows(p) ? dispatch_split<T, 16 / sizeof(T), false>(p, rms, nullptr, nullptr, stream)
+                          : dispatch_split<T, 1, false>(p, rms, nullptr, nullptr, stream);
 }
 
-// Blocks of the backward pass, which is also the number of partial rows in the workspace.
-inline int backward_blocks(long long rows, int channels) {
-    if (channels > kMaxNarrow) {
-        return static_cast<int>(std::max(1LL, std::min((rows + 31) / 32, 148LL * 2)));
-    }
-    return static_cast<int>(std::max(1LL, std::min((rows + kWarps - 1) / kWarps, 148LL * 2)));
+// Partial rows that the backward pass may write.
+inline int partial_rows(long long rows) {
+    return static_cast<int>(std::max(1LL, std::min<long long>((rows + kWarps - 1) / kWarps, kMaxBackwardBlocks)));
 }
 
 template <typename T>
-int run_backward(NormArgs<T> p, bool rms, T* dw, T* db, cudaStream_t stream) {
-    int blocks = backward_blocks(p.rows, p.channels);
-    int code;
-    if (p.channels > kMaxNarrow) {
-        const int grid = static_cast<int>(std::min(p.rows, 148LL * 8));
-        if (rms) {
-            norm_backward_wide_kernel<T, true><<<grid, kThreads, 0, stream>>>(p);
-        } else {
-            norm_backward_wide_kernel<T, false><<<grid, kThreads, 0, stream>>>(p);
-        }
-        LAT_LAUNCH_CHECK();
-        if (p.partial == nullptr) {
-            return LAT_OK;
-        }
-        const long long per_block = (p.rows + blocks - 1) / blocks;
-        blocks = static_cast<int>((p.rows + per_block - 1) / per_block);
-        const dim3 sums_grid(blocks, (p.channels + kThreads - 1) / kThreads);
-        if (rms) {
-            norm_sums_wide_kernel<T, true><<<sums_grid, kThreads, 0, stream>>>(p, per_block);
-        } else {
-            norm_sums_wide_kernel<T, false><<<sums_grid, kThreads, 0, stream>>>(p, per_block);
-        }
-        LAT_LAUNCH_CHECK();
-    } else {
-        const bool vec = vector_rows(p);
-        int lanes, k;
-        split_row(vec ? p.channels * static_cast<int>(sizeof(T)) / 16 : p.channels,
-                  vec ? kMaxLaneElements * static_cast<int>(sizeof(T)) / 16 : kMaxLaneElements, lanes, k);
-        blocks = std::min(blocks, norm_grid(p.rows, lanes));
-        code = vec ? dispatch_split<T, 16 / sizeof(T)>(p, rms, blocks, stream)
-                   : dispatch_split<T, 1>(p, rms, blocks, stream);
-        if (code != LAT_OK || p.partial == nullptr) {
-            return code;
-        }
+int run_backward(const NormArgs<T>& p, bool rms, T* dw, T* db, cudaStream_t stream) {
+    if (p.channels <= kMaxNarrow) {
+        return vector_rows(p) ? dispatch_split<T, 16 / sizeof(T), true>(p, rms, dw, db, stream)
+                              : dispatch_split<T, 1, true>(p, rms, dw, db, stream);
     }
-    norm_reduce_kernel<T><<<(2 * p.channels + 31) / 32, kThreads, 0, stream>>>(
-        p.partial, blocks, p.channels, dw, db);
+    const int grid = static_cast<int>(std::min(p.rows, 148LL * 8));
+    if (rms) {
+        norm_backward_wide_kernel<T, true><<<grid, kThreads, 0, stream>>>(p);
+    } else {
+        norm_backward_wide_kernel<T, false><<<grid, kThreads, 0, stream>>>(p);
+    }
     LAT_LAUNCH_CHECK();
-    return LAT_OK;
+    if (dw == nullptr && db == nullptr) {
+        return LAT_OK;
+    }
+    const long long per_block = (p.rows + partial_rows(p.rows) - 1) / partial_rows(p.rows);
+    const int blocks = static_cast<int>((p.rows + per_block - 1) / per_block);
+    const dim3 sums_grid(blocks, (p.channels + kThreads - 1) / kThreads);
+    LAT_REQUIRE(sums_grid.y <= 65535, "normalisation supports at most 16 million channels.");
+    if (rms) {
+        norm_sums_wide_kernel<T, true><<<sums_grid, kThreads, 0, stream>>>(p, per_block);
+    } else {
+        norm_sums_wide_kernel<T, false><<<sums_grid, kThreads, 0, stream>>>(p, per_block);
+    }
+    LAT_LAUNCH_CHECK();
+    return launch_reduce(p, blocks, dw, db, stream);
 }
 
 template <typename T>
@@ -561,7 +605,7 @@ size_t lat_row_norm_backward_workspace_bytes(int64_t rows, int32_t channels) {
     if (rows <= 0 || channels <= 0) {
         return 256;
     }
-    return align_up(sizeof(float) * 2 * static_cast<size_t>(channels) * backward_blocks(rows, channels));
+    return align_up(sizeof(float) * 2 * static_cast<size_t>(channels) * partial_rows(rows));
 }
 
 int lat_row_norm_backward(

@@ -62,7 +62,7 @@ def test_recurrence_entry_points_refuse_bad_arguments():
     _refused(forward(offsets=None), 'offsets')
     _refused(forward(offsets=None, sequences=0), 'offsets')
     _refused(forward(x=None), 'shape (N, C)')
-    need = lib.lat_recurrence_workspace_bytes(300, 8)
+    need = lib.lat_recurrence_workspace_bytes(F32, 300, 8)
     assert forward(rows=300, ws=buf, ws_bytes=need - 1) == _native.LAT_WORKSPACE_TOO_SMALL
     assert forward(rows=300) == _native.LAT_WORKSPACE_TOO_SMALL
     assert forward(rows=0, x=None, offsets=None, sequences=0) == _native.LAT_OK
@@ -70,7 +70,7 @@ def test_recurrence_entry_points_refuse_bad_arguments():
                                          None, 0, None, None), 'tile states')
     _refused(lib.lat_recurrence_step(F32, buf, 8, buf, 8, None, 4, 8, buf, buf, None), 'state must have shape')
     _refused(lib.lat_recurrence_step(F32, buf, 8, buf, 8, buf, 4, 0, buf, buf, None), 'shape (N, C)')
-    assert [lib.lat_recurrence_tiles(n) for n in (-1, 0, 1, 128, 129)] == [0, 0, 1, 1, 2]
+    assert [lib.lat_recurrence_carry_rows(n) for n in (-1, 0, 1, 8, 9)] == [0, 0, 1, 1, 2]
 
 
 def test_host_tensors_are_refused():
