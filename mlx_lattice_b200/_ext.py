@@ -15,7 +15,7 @@ from typing import Sequence
 import torch
 
 from mlx_lattice_b200 import _native
-from mlx_lattice_b200._native import FloatTriple, Triple, check
+from mlx_lattice_b200._native import FloatTriple, Triple, bindings, check
 
 _REDUCE = {'sum': 0, 'max': 1, 'avg': 2}
 _JOIN = {'inner': 0, 'left': 1, 'right': 2, 'outer': 3}
@@ -1156,120 +1156,33 @@ def row_norm(feats, weight, bias, eps: float, rms: bool):
     return out
 
 
+# The operators below have gradients; their argument checks, output tensors and autograd nodes
+# are in ``csrc/bindings.cpp``.
+
+
 def row_norm_forward(feats, weight, bias, eps: float, rms: bool):
     """``row_norm`` for training: ``(out, mean, rstd)`` with the float32 row statistics that
     ``row_norm_backward`` takes (``mean`` is None for the RMS form)."""
-    feats, stride = _feats_arg(feats)
-    dtype = _dtype_code(feats.dtype)
-    rows, channels = int(feats.shape[0]), int(feats.shape[1])
-    device = feats.device
-    weight, bias = _vec_arg(weight, 'weight', channels, feats), _vec_arg(bias, 'bias', channels, feats)
-    out = torch.empty((rows, channels), dtype=feats.dtype, device=device)
-    mean = None if rms else torch.empty(rows, dtype=torch.float32, device=device)
-    rstd = torch.empty(rows, dtype=torch.float32, device=device)
-    with torch.cuda.device(device):
-        check(_lib().lat_row_norm_forward(
-            dtype, int(bool(rms)), _ptr(feats), rows, channels, stride, _ptr(weight), _ptr(bias), float(eps),
-            _ptr(out), _ptr(mean), _ptr(rstd), _stream(),
-        ))
-    return out, mean, rstd
+    return bindings().row_norm_forward(feats, weight, bias, eps, rms)
 
 
 def row_norm_backward(grad, feats, weight, mean, rstd, rms: bool, want_weight: bool, want_bias: bool):
     """Gradients of ``row_norm_forward``: ``(grad_feats, grad_weight, grad_bias)``, the last two
     None unless wanted."""
-    feats, stride = _feats_arg(feats)
-    grad, grad_stride = _grad_arg(grad, feats)
-    dtype = _dtype_code(feats.dtype)
-    rows, channels = int(feats.shape[0]), int(feats.shape[1])
-    device = feats.device
-    weight = _vec_arg(weight, 'weight', channels, feats)
-    mean = None if rms else _vec_arg(mean, 'mean', rows, feats, torch.float32)
-    rstd = _vec_arg(rstd, 'rstd', rows, feats, torch.float32)
-    grad_feats = torch.empty((rows, channels), dtype=feats.dtype, device=device)
-    grad_weight = torch.empty(channels, dtype=feats.dtype, device=device) if want_weight else None
-    grad_bias = torch.empty(channels, dtype=feats.dtype, device=device) if want_bias else None
-    lib = _lib()
-    ws = (_workspace(lib.lat_row_norm_backward_workspace_bytes(rows, channels), device)
-          if want_weight or want_bias else None)
-    with torch.cuda.device(device):
-        check(lib.lat_row_norm_backward(
-            dtype, int(bool(rms)), _ptr(grad), grad_stride, _ptr(feats), rows, channels, stride, _ptr(weight),
-            _ptr(mean), _ptr(rstd), _ptr(grad_feats), _ptr(grad_weight), _ptr(grad_bias), _ptr(ws),
-            0 if ws is None else ws.numel(), _stream(),
-        ))
-    return grad_feats, grad_weight, grad_bias
+    return bindings().row_norm_backward(grad, feats, weight, mean, rstd, rms, want_weight, want_bias)
 
 
-def _grad_arg(grad, feats):
-    _require_cuda(grad, 'grad')
-    if grad.device != feats.device or grad.dtype != feats.dtype or grad.shape != feats.shape:
-        raise ValueError('grad must match the features in shape, dtype and device.')
-    return _feats_arg(grad)
+def row_norm_recorded(feats, weight, bias, eps: float, rms: bool):
+    """The normalised features recorded for a gradient; None where no argument asks for one."""
+    return bindings().row_norm_recorded(feats, weight, bias, eps, rms)
 
 
 def dropout(feats, p: float, seed, offset: int = 0, residual=None):
     """``feats`` with elements dropped at probability ``p`` and the others scaled by
     ``1 / (1 - p)``, plus ``residual``; the mask is a function of ``seed``, ``offset`` and the
     element's place. ``seed`` is an int, or an int64 CUDA tensor of one element that is read
-    when the kernel runs."""
-    feats, _ = _feats_arg(feats)
-    feats = feats.contiguous()
-    dtype = _dtype_code(feats.dtype)
-    if not 0 <= p < 1:
-        raise ValueError('p must satisfy 0 <= p < 1.')
-    device = feats.device
-    if residual is not None:
-        _require_cuda(residual, 'residual')
-        if residual.shape != feats.shape or residual.dtype != feats.dtype or residual.device != device:
-            raise ValueError('residual must match the features in shape, dtype and device.')
-        residual = residual.contiguous()
-    word = None
-    if isinstance(seed, torch.Tensor):
-        if not seed.is_cuda or seed.device != device or seed.dtype != torch.int64 or seed.numel() != 1:
-            raise ValueError('seed must be an int or an int64 CUDA tensor of one element on the feature device.')
-        word, seed = seed, 0
-    out = torch.empty_like(feats)
-    with torch.cuda.device(device):
-        check(_lib().lat_dropout(
-            dtype, _ptr(feats), _ptr(residual), feats.numel(), float(p), int(seed) & _WORD, _ptr(word),
-            int(offset) & _WORD, _ptr(out), _stream(),
-        ))
-    return out
-
-
-_WORD = (1 << 64) - 1
-
-
-# --------------------------------------------------------------------------- #
-# gated linear recurrence over the rows of each sequence
-# --------------------------------------------------------------------------- #
-
-
-def _recurrence_args(feats, gate):
-    feats, stride = _feats_arg(feats)
-    dtype = _dtype_code(feats.dtype)
-    _require_cuda(gate, 'gate')
-    if gate.shape != feats.shape or gate.dtype != feats.dtype or gate.device != feats.device:
-        raise ValueError('gate must match the features in shape, dtype and device.')
-    gate, gate_stride = _feats_arg(gate)
-    return feats, stride, gate, gate_stride, dtype
-
-
-def _state_arg(state, name: str, rows: int, channels: int, device):
-    if state is None:
-        return None
-    _require_cuda(state, name)
-    if tuple(state.shape) != (rows, channels) or state.dtype != torch.float32 or state.device != device:
-        raise ValueError(f'{name} must have shape ({rows}, {channels}) and float32 dtype on the feature device.')
-    return state.contiguous()
-
-
-def _offsets_arg(offsets, device):
-    offsets = _i32(offsets, 'offsets')
-    if offsets.ndim != 1 or offsets.numel() < 1 or offsets.device != device:
-        raise ValueError('offsets must hold one int32 entry per sequence and one more, on the feature device.')
-    return offsets, int(offsets.numel()) - 1
+    when the kernel runs. Differentiable in ``feats`` and ``residual``."""
+    return bindings().dropout(feats, p, seed, offset, residual)
 
 
 def recurrence_forward(feats, gate, offsets, initial_state=None, reverse: bool = False, *,
@@ -1277,74 +1190,34 @@ def recurrence_forward(feats, gate, offsets, initial_state=None, reverse: bool =
     """``h_t = a_t h_{t-1} + (1 - a_t) feats_t`` with ``a = sigmoid(gate)`` over the rows of each
     sequence: ``(h, final_state, carries)``, the last two None unless wanted. ``carries`` is
     what ``recurrence_backward`` takes."""
-    feats, stride, gate, gate_stride, dtype = _recurrence_args(feats, gate)
-    rows, channels = int(feats.shape[0]), int(feats.shape[1])
-    device = feats.device
-    offsets, sequences = _offsets_arg(offsets, device)
-    initial_state = _state_arg(initial_state, 'initial_state', sequences, channels, device)
-    out = torch.empty((rows, channels), dtype=feats.dtype, device=device)
-    lib = _lib()
-    final = torch.empty((sequences, channels), dtype=torch.float32, device=device) if want_state else None
-    carries = (torch.empty((lib.lat_recurrence_carry_rows(rows), channels), dtype=torch.float32, device=device)
-               if want_carries else None)
-    ws = _workspace(lib.lat_recurrence_workspace_bytes(dtype, rows, channels), device)
-    with torch.cuda.device(device):
-        check(lib.lat_recurrence_forward(
-            dtype, _ptr(feats), stride, _ptr(gate), gate_stride, rows, channels, _ptr(offsets), sequences,
-            _ptr(initial_state), int(bool(reverse)), _ptr(out), _ptr(final), _ptr(carries), _ptr(ws), ws.numel(),
-            _ptr(status_word(device)), _stream(),
-        ))
-    return out, final, carries
+    _require_cuda(feats, 'feats')
+    return bindings().recurrence_forward(
+        feats, gate, offsets, initial_state, reverse, want_state, want_carries, status_word(feats.device))
 
 
 def recurrence_backward(grad, grad_final, feats, gate, offsets, initial_state, reverse: bool, carries, *,
                         want_initial: bool = False):
     """Gradients of ``recurrence_forward``: ``(grad_feats, grad_gate, grad_initial)``, the last
     one None unless wanted. ``grad_final`` may be None."""
-    feats, stride, gate, gate_stride, dtype = _recurrence_args(feats, gate)
-    grad, grad_stride = _grad_arg(grad, feats)
-    rows, channels = int(feats.shape[0]), int(feats.shape[1])
-    device = feats.device
-    offsets, sequences = _offsets_arg(offsets, device)
-    initial_state = _state_arg(initial_state, 'initial_state', sequences, channels, device)
-    grad_final = _state_arg(grad_final, 'grad_final', sequences, channels, device)
-    lib = _lib()
-    carries = _state_arg(carries, 'carries', lib.lat_recurrence_carry_rows(rows), channels, device)
-    grad_feats = torch.empty((rows, channels), dtype=feats.dtype, device=device)
-    grad_gate = torch.empty((rows, channels), dtype=feats.dtype, device=device)
-    grad_initial = torch.empty((sequences, channels), dtype=torch.float32, device=device) if want_initial else None
-    ws = _workspace(lib.lat_recurrence_workspace_bytes(dtype, rows, channels), device)
-    with torch.cuda.device(device):
-        check(lib.lat_recurrence_backward(
-            dtype, _ptr(grad), grad_stride, _ptr(grad_final), _ptr(feats), stride, _ptr(gate), gate_stride, rows,
-            channels, _ptr(offsets), sequences, _ptr(initial_state), int(bool(reverse)), _ptr(carries),
-            _ptr(grad_feats), _ptr(grad_gate), _ptr(grad_initial), _ptr(ws), ws.numel(),
-            _ptr(status_word(device)), _stream(),
-        ))
-    return grad_feats, grad_gate, grad_initial
+    _require_cuda(feats, 'feats')
+    return bindings().recurrence_backward(
+        grad, grad_final, feats, gate, offsets, initial_state, reverse, carries, want_initial,
+        status_word(feats.device))
+
+
+def recurrence(feats, gate, offsets, initial_state=None, reverse: bool = False, *, want_state: bool = False):
+    """``(h, final_state)`` of ``recurrence_forward``, differentiable in ``feats``, ``gate`` and
+    ``initial_state``; the state is None unless wanted."""
+    _require_cuda(feats, 'feats')
+    return bindings().recurrence(
+        feats, gate, offsets, initial_state, reverse, want_state, status_word(feats.device))
 
 
 def recurrence_step(feats, gate, state, out_state=None):
     """One row of every stream: ``(h, next_state)`` with ``next_state = a state + (1 - a) feats``
     in float32 and ``h`` the same in the feature dtype. ``out_state`` (optional) receives the
     next state and may be ``state`` itself."""
-    feats, stride, gate, gate_stride, dtype = _recurrence_args(feats, gate)
-    rows, channels = int(feats.shape[0]), int(feats.shape[1])
-    device = feats.device
-    if state is None:
-        raise ValueError('state must have shape (N, C) and float32 dtype on the feature device.')
-    state = _state_arg(state, 'state', rows, channels, device)
-    if out_state is None:
-        out_state = torch.empty((rows, channels), dtype=torch.float32, device=device)
-    elif _state_arg(out_state, 'out_state', rows, channels, device) is not out_state:
-        raise ValueError('out_state must be contiguous.')
-    out = torch.empty((rows, channels), dtype=feats.dtype, device=device)
-    with torch.cuda.device(device):
-        check(_lib().lat_recurrence_step(
-            dtype, _ptr(feats), stride, _ptr(gate), gate_stride, _ptr(state), rows, channels, _ptr(out),
-            _ptr(out_state), _stream(),
-        ))
-    return out, out_state
+    return bindings().recurrence_step(feats, gate, state, out_state)
 
 
 def relu(feats):

@@ -7,6 +7,7 @@ calling them without an sm_100 GPU, raises.
 from __future__ import annotations
 
 import ctypes
+import importlib
 import os
 from ctypes import (
     POINTER, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_uint64, c_void_p,
@@ -128,6 +129,7 @@ SIGNATURES = {
 }
 
 _lib = None
+_bindings = None
 
 
 def library_present() -> bool:
@@ -151,6 +153,22 @@ def load() -> ctypes.CDLL:
         fn.argtypes = argtypes
     _lib = lib
     return lib
+
+
+def bindings():
+    """The torch side of the differentiable operators (``_bindings.so``). Raises if it is not
+    built."""
+    global _bindings
+    if _bindings is None:
+        load()
+        try:
+            _bindings = importlib.import_module('mlx_lattice_b200._bindings')
+        except ImportError as error:
+            raise RuntimeError(
+                'mlx_lattice_b200/_bindings.so is not built or does not load; run '
+                f'`python -m mlx_lattice_b200.build`. ({error})'
+            ) from error
+    return _bindings
 
 
 def last_error() -> str:

@@ -6,7 +6,6 @@ import torch
 
 from mlx_lattice_b200 import _ext
 from mlx_lattice_b200.core import QuantizedWeight, SparseTensor
-from mlx_lattice_b200.ops import _autograd
 from mlx_lattice_b200.ops._quantized import quantized_matmul
 
 __all__ = [
@@ -96,11 +95,7 @@ def dropout(
         if residual is None:
             return x.replace(feats=x.feats)
         p, seed = 0.0, 0
-    if _autograd.wanted(x.feats, residual):
-        feats = _autograd.Dropout.apply(x.feats, residual, float(p), seed, int(offset))
-    else:
-        feats = _ext.dropout(x.feats, p, seed, offset, residual)
-    return x.replace(feats=feats)
+    return x.replace(feats=_ext.dropout(x.feats, p, seed, offset, residual))
 
 
 def layer_norm(x: SparseTensor, *, weight=None, bias=None, eps: float = 1e-5) -> SparseTensor:
@@ -108,9 +103,10 @@ def layer_norm(x: SparseTensor, *, weight=None, bias=None, eps: float = 1e-5) ->
     Differentiable in ``x.feats``, ``weight`` and ``bias``."""
     if eps <= 0:
         raise ValueError('eps must be positive.')
-    if _autograd.wanted(x.feats, weight, bias):
-        return x.replace(feats=_autograd.RowNorm.apply(x.feats, weight, bias, float(eps), False))
-    return x.replace(feats=_ext.row_norm(x.feats, weight, bias, eps, rms=False))
+    feats = _ext.row_norm_recorded(x.feats, weight, bias, eps, rms=False)
+    if feats is None:
+        feats = _ext.row_norm(x.feats, weight, bias, eps, rms=False)
+    return x.replace(feats=feats)
 
 
 def rms_norm(x: SparseTensor, *, weight=None, eps: float = 1e-5) -> SparseTensor:
@@ -118,9 +114,10 @@ def rms_norm(x: SparseTensor, *, weight=None, eps: float = 1e-5) -> SparseTensor
     ``x.feats`` and ``weight``."""
     if eps <= 0:
         raise ValueError('eps must be positive.')
-    if _autograd.wanted(x.feats, weight):
-        return x.replace(feats=_autograd.RowNorm.apply(x.feats, weight, None, float(eps), True))
-    return x.replace(feats=_ext.row_norm(x.feats, weight, None, eps, rms=True))
+    feats = _ext.row_norm_recorded(x.feats, weight, None, eps, rms=True)
+    if feats is None:
+        feats = _ext.row_norm(x.feats, weight, None, eps, rms=True)
+    return x.replace(feats=feats)
 
 
 def batch_norm(

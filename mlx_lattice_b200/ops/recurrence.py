@@ -7,7 +7,6 @@ import torch
 
 from mlx_lattice_b200 import _ext
 from mlx_lattice_b200.core import SparseTensor
-from mlx_lattice_b200.ops import _autograd
 
 __all__ = ['gated_recurrence', 'gated_recurrence_step', 'sequence_offsets']
 
@@ -39,12 +38,7 @@ def gated_recurrence(
     gate = _gate(x, gate)
     if offsets is None:
         offsets = sequence_offsets(x)
-    if _autograd.wanted(x.feats, gate, initial_state):
-        h, final = _autograd.GatedRecurrence.apply(
-            x.feats, gate, initial_state, offsets, bool(reverse), bool(return_state))
-    else:
-        h, final, _ = _ext.recurrence_forward(
-            x.feats, gate, offsets, initial_state, reverse, want_state=return_state)
+    h, final = _ext.recurrence(x.feats, gate, offsets, initial_state, reverse, want_state=return_state)
     h = x.replace(feats=h)
     return (h, final) if return_state else h
 

@@ -83,6 +83,12 @@ def test_host_tensors_are_refused():
             call()
 
 
+def test_exceptions_pass_through_the_bindings():
+    """An exception thrown inside the extension itself reaches Python."""
+    with pytest.raises(TypeError, match='integer'):
+        _ext.dropout(torch.zeros((4, 8)), 0.5, 'seed')
+
+
 def test_module_arguments():
     with pytest.raises(ValueError, match='0 <= p < 1'):
         nn.Dropout(1.0)
