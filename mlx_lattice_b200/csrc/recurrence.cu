@@ -177,6 +177,20 @@ struct Cursor {
         settle(order);
     }
 
+    // the sequence before, where there is one
+    __device__ __forceinline__ bool back(const Order& order) {
+        for (int k = j - 1; k >= 0; --k) {
+            const int b = order.begin(k), e = order.begin(k + 1);
+            if (e > b) {
+                j = k;
+                begin = b;
+                end = e;
+                return true;
+            }
+        }
+        return false;
+    }
+
     // no sequence starts or ends among these rows, which all belong to this one
     __device__ __forceinline__ bool covers(int first, int rows) const { return begin < first && end > first + rows; }
 };
@@ -258,6 +272,10 @@ template <typename T, bool Whole, bool Backward> struct Walk {
         row_step = p.order.reverse ? -1 : 1;
     }
 
+    __device__ __forceinline__ const T* row(const T* from, long long stride, const Order& order, int row) const {
+        return from + order.row(row) * stride + c;
+    }
+
     // to: the thread's first channel in the row
     __device__ __forceinline__ void store(T* to, const Row<T>& value) const {
         Stored<T> raw;
@@ -333,14 +351,11 @@ template <typename T, bool Whole, int Arrays, int Rows, int Stages> struct Ring 
         return reinterpret_cast<Stored<T>*>(ring) + ((stage * Arrays + array) * Rows + row) * kThreads + threadIdx.x;
     }
 
-    // Rows first .. first + Rows - 1; zeros from row `end` on and for channels that do not exist.
+    // `rows` more rows, at most Rows, from `at` on, which moves on to the row behind them; zeros
+    // for rows and channels that do not exist.
     template <typename W>
-    __device__ __forceinline__ void fetch(
-        const W& walk, int stage, int array, const T* from, long long stride, const Order& order, int first, int end
-    ) const {
-        const T* at = from + order.row(first) * stride + walk.c;
-        const long long step = walk.row_step * stride;
-        if (Whole && first + Rows <= end) {
+    __device__ __forceinline__ void fetch(const W& walk, int stage, int array, const T*& at, long long step, int rows) const {
+        if (Whole && rows >= Rows) {
             const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot(stage, array, 0)));
 #pragma unroll
             for (int r = 0; r < Rows; ++r) {
@@ -352,7 +367,7 @@ template <typename T, bool Whole, int Arrays, int Rows, int Stages> struct Ring 
                 Stored<T> raw;
 #pragma unroll
                 for (int i = 0; i < kWide<T>; ++i) {
-                    raw.v[i] = first + r < end && i < walk.count ? at[i] : narrow<T>(0.0f);
+                    raw.v[i] = r < rows && i < walk.count ? at[i] : narrow<T>(0.0f);
                 }
                 *slot(stage, array, r) = raw;
                 at += step;
@@ -427,12 +442,13 @@ template <bool Value> struct Flag {
     static constexpr bool value = Value;
 };
 
-// One row of the recurrence.
+// One row of the recurrence, as h = x + a (h - x): the weights of h and x add up to one whatever
+// the rounding of a, so a long memory does not gather it.
 template <typename T>
 __device__ __forceinline__ void advance(Row<T>& h, const Row<T>& a, const Row<T>& x) {
 #pragma unroll
     for (int i = 0; i < Row<T>::kPairs; ++i) {
-        h.v[i] = fma(a.v[i], h.v[i], minus(both(1.0f), a.v[i]) * x.v[i]);
+        h.v[i] = fma(a.v[i], minus(h.v[i], x.v[i]), x.v[i]);
     }
 }
 
@@ -445,10 +461,10 @@ template <typename T> __device__ __forceinline__ Row<T> gates(const Row<T>& z) {
     return a;
 }
 
-constexpr int kRingRows = 4, kRingStages = 4;
+constexpr int kRingRows = 4, kRingStages = 3;
 
 template <typename T, bool Whole>
-__global__ void __launch_bounds__(kThreads, 3) recurrence_maps_kernel(ScanArgs<T> p) {
+__global__ void __launch_bounds__(kThreads, 4) recurrence_maps_kernel(ScanArgs<T> p) {
     constexpr int R = kRingRows, S = kRingStages;
     const Walk<T, Whole, false> walk(p, blockIdx.x);
     const Ring<T, Whole, 2, R, S> ring;
@@ -456,10 +472,12 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_maps_kernel(ScanArgs<T
     bool cut = false;
     if (walk.count > 0) {
         const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
+        const T* from = walk.row(p.x, p.x_stride, p.order, first);
+        const T* gates_from = walk.row(p.z, p.z_stride, p.order, first);
         const auto fetch = [&](int row, int stage) {
             if (row < end) {
-                ring.fetch(walk, stage, 0, p.x, p.x_stride, p.order, row, end);
-                ring.fetch(walk, stage, 1, p.z, p.z_stride, p.order, row, end);
+                ring.fetch(walk, stage, 0, from, walk.row_step * p.x_stride, end - row);
+                ring.fetch(walk, stage, 1, gates_from, walk.row_step * p.z_stride, end - row);
             }
             ring.commit();
         };
@@ -509,7 +527,7 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_maps_kernel(ScanArgs<T
 }
 
 template <typename T, bool Whole>
-__global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<T> p) {
+__global__ void __launch_bounds__(kThreads, 4) recurrence_apply_kernel(ScanArgs<T> p) {
     constexpr int R = kRingRows, S = kRingStages;
     // the last tiles first: the maps kernel read them last
     const int block = gridDim.x - 1 - blockIdx.x;
@@ -520,10 +538,12 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<
         return;
     }
     const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
+    const T* from = walk.row(p.x, p.x_stride, p.order, first);
+    const T* gates_from = walk.row(p.z, p.z_stride, p.order, first);
     const auto fetch = [&](int row, int stage) {
         if (row < end) {
-            ring.fetch(walk, stage, 0, p.x, p.x_stride, p.order, row, end);
-            ring.fetch(walk, stage, 1, p.z, p.z_stride, p.order, row, end);
+            ring.fetch(walk, stage, 0, from, walk.row_step * p.x_stride, end - row);
+            ring.fetch(walk, stage, 1, gates_from, walk.row_step * p.z_stride, end - row);
         }
         ring.commit();
     };
@@ -578,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<
 // of the same kind backwards in time. A tile's map needs no walk backwards: what it hands out is
 // the sum of its dy_t times the product of its gates up to t, as far as the first sequence's end.
 template <typename T, bool Whole>
-__global__ void __launch_bounds__(kThreads, 3) recurrence_flow_maps_kernel(ScanArgs<T> p) {
+__global__ void __launch_bounds__(kThreads, 4) recurrence_flow_maps_kernel(ScanArgs<T> p) {
     constexpr int R = kRingRows, S = kRingStages;
     const Walk<T, Whole, true> walk(p, blockIdx.x);
     const Ring<T, Whole, 2, R, S> ring;
@@ -586,10 +606,12 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_flow_maps_kernel(ScanA
     bool open = true;
     if (walk.count > 0) {
         const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
+        const T* from = walk.row(p.dy, p.dy_stride, p.order, first);
+        const T* gates_from = walk.row(p.z, p.z_stride, p.order, first);
         const auto fetch = [&](int row, int stage) {
             if (row < end) {
-                ring.fetch(walk, stage, 0, p.dy, p.dy_stride, p.order, row, end);
-                ring.fetch(walk, stage, 1, p.z, p.z_stride, p.order, row, end);
+                ring.fetch(walk, stage, 0, from, walk.row_step * p.dy_stride, end - row);
+                ring.fetch(walk, stage, 1, gates_from, walk.row_step * p.z_stride, end - row);
             }
             ring.commit();
         };
@@ -654,22 +676,34 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
     const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
     const auto fetch = [&](int row, int stage) {
         if (row >= first) {
-            ring.fetch(walk, stage, 0, p.x, p.x_stride, p.order, row, end);
-            ring.fetch(walk, stage, 1, p.z, p.z_stride, p.order, row, end);
-            ring.fetch(walk, stage, 2, p.dy, p.dy_stride, p.order, row, end);
+            const T* x = walk.row(p.x, p.x_stride, p.order, row);
+            const T* z = walk.row(p.z, p.z_stride, p.order, row);
+            const T* dy = walk.row(p.dy, p.dy_stride, p.order, row);
+            ring.fetch(walk, stage, 0, x, walk.row_step * p.x_stride, end - row);
+            ring.fetch(walk, stage, 1, z, walk.row_step * p.z_stride, end - row);
+            ring.fetch(walk, stage, 2, dy, walk.row_step * p.dy_stride, end - row);
         }
         ring.commit();
     };
     const int last = first + (end - 1 - first) / R * R;
     fetch(last, 0);
     Row<T> e = reaching_state<T>(p, walk, block);
+    Cursor cursor;
+    cursor.seek(p.order, last);
     const long long down = walk.row_step * p.channels;
     int stage = 0;
 #pragma unroll 1
     for (int row = last; row >= first; row -= R) {
         Row<T> h = walk.state(p.carries, row / R, p.channels);
-        Cursor cursor;
-        cursor.seek(p.order, row);
+        // from the sequence of the batch behind, or the one after it, back to the first that ends
+        // behind this batch's first row
+        while (cursor.begin > row) {
+            Cursor before = cursor;
+            if (!before.back(p.order) || before.end <= row) {
+                break;
+            }
+            cursor = before;
+        }
         const bool covered = cursor.covers(row, R);
         // of the batch's rows: start a sequence, end one, lie outside all
         unsigned heads = 0, tails = 0, dead = 0;
@@ -708,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
 #pragma unroll
             for (int r = R - 1; r >= 0; --r) {
                 if (decltype(marked)::value && (tails >> r & 1u)) {
-                    cursor.seek(p.order, row + r);
+                    cursor.back(p.order);
                     e = walk.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
                 }
                 const Row<T> up = ring.row(stage, 2, r);
@@ -727,7 +761,6 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
                     walk.store(p.dz + at0 + r * down, dz);
                 }
                 if (decltype(marked)::value && (heads >> r & 1u)) {
-                    cursor.seek(p.order, row + r);
                     walk.store_state(p.dinitial, p.order.sequence(cursor.j), p.channels, e);
                 }
             }
@@ -801,7 +834,7 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(
 #pragma unroll
     for (int i = 0; i < V; ++i) {
         const float a = sigmoid_gate(zs.get(i));
-        now.v[i] = fmaf(a, old.v[i], (1.0f - a) * xs.get(i));
+        now.v[i] = fmaf(a, old.v[i] - xs.get(i), xs.get(i));
         y.set(i, now.v[i]);
     }
     store_pack<T, V>(h + row * channels + c, y);
