@@ -8,8 +8,7 @@
 //   dx_t = (1 - a_t) dh_t,  dz_t = a_t (1 - a_t) dh_t (h_{t-1} - x_t),  dinitial = a_1 dh_1
 //
 // Both directions are scans over affine maps h -> A h + H, which compose associatively. The
-// rows are cut into tiles of 64; a thread walks one tile for eight bytes of channels. Three
-// kernels:
+// rows are cut into tiles of 32; a thread walks a tile for 16 bytes of channels. Three kernels:
 //   maps:   the map (A, H) of every tile, and for a group of tiles (a block) the maps of the
 //           tiles before each one in the group and of the whole group
 //   scan:   the state that reaches every group, from the groups' maps
@@ -34,11 +33,13 @@ namespace lat {
 
 namespace {
 
-constexpr int kTileRows = 64;
+constexpr int kTileRows = 32;
 constexpr int kThreads = 256;
+constexpr int kMapBytes = 16;                 // channels of a thread of the maps and apply kernels
+constexpr int kGradientBytes = 8;             // of the gradient kernel, which keeps twice as much of each
+constexpr int kGradientTiles = 2;             // that a thread of the gradient kernel walks through
 constexpr float kReset = -1.0f;
 constexpr int kCarryRows = 8;                 // rows from one kept state to the next
-template <typename T> constexpr int kWide = 8 / static_cast<int>(sizeof(T));   // channels of a thread
 
 // later after earlier, as maps
 __device__ __forceinline__ float2 compose(float2 earlier, float2 later) {
@@ -202,8 +203,9 @@ template <typename T> struct ScanArgs {
     long long x_stride, z_stride, dy_stride;
     Order order;
     int channels;
-    int slabs;              // of kWide * lanes channels
-    int lanes;              // threads across a slab, eight bytes each
+    int slabs;              // of the kernel's launch: lanes times a thread's channels
+    int lanes;              // threads across a slab
+    int per_group;          // tiles of a group
     int tiles;
     const float* initial;   // [sequences][channels] or null
     float2* maps;           // [tiles][channels] of the tiles before in the group
@@ -219,14 +221,14 @@ template <typename T> struct ScanArgs {
     int32_t* status;
 };
 
-// The channels of a thread in one row, as they are stored ...
-template <typename T> struct alignas(8) Stored {
-    T v[kWide<T>];
+// N channels of a row, as they are stored ...
+template <typename T, int N> struct alignas(N * sizeof(T)) Stored {
+    T v[N];
 };
 
 // ... and as float pairs.
-template <typename T> struct Row {
-    static constexpr int kPairs = kWide<T> / 2;
+template <int N> struct Row {
+    static constexpr int kPairs = N / 2;
     Pair v[kPairs];
 
     static __device__ __forceinline__ Row filled(float value) {
@@ -238,7 +240,7 @@ template <typename T> struct Row {
         return out;
     }
 
-    static __device__ __forceinline__ Row from(const Stored<T>& raw) {
+    template <typename T> static __device__ __forceinline__ Row from(const Stored<T, N>& raw) {
         Row out;
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
@@ -256,19 +258,18 @@ template <typename T> struct Row {
     __device__ __forceinline__ void set(int i, float value) { (i % 2 == 0 ? v[i / 2].x : v[i / 2].y) = value; }
 };
 
-// A thread's place: its tile and its channels c .. c + count - 1, at most kWide. Tiles are
-// numbered in the order of the chain (`place`): of time, or backwards in time for the gradient.
-// Whole: channels come in full eights of bytes and can be moved at once.
-template <typename T, bool Whole, bool Backward> struct Walk {
-    int place, tile, c, count;
+// Channels c .. c + count - 1 of a thread, at most N, and how they move. Granule: the bytes that
+// move at once, as alignment and channel count allow; 0: one element.
+template <typename T, int N, int Granule> struct Channels {
+    static constexpr int kBytes = N * static_cast<int>(sizeof(T));
+    static constexpr int kMove = Granule == 0 ? static_cast<int>(sizeof(T)) : Granule < kBytes ? Granule : kBytes;
+    static constexpr int kMoveChannels = kMove / static_cast<int>(sizeof(T));
+    int c, count;
     long long row_step;   // from a row to the next one, in rows of an array
 
-    __device__ __forceinline__ Walk(const ScanArgs<T>& p, int block) {
-        const int group = block / p.slabs, slab = block - group * p.slabs;
-        place = group * (kThreads / p.lanes) + static_cast<int>(threadIdx.x) / p.lanes;
-        tile = Backward ? p.tiles - 1 - place : place;
-        c = (slab * p.lanes + static_cast<int>(threadIdx.x) % p.lanes) * kWide<T>;
-        count = place < p.tiles ? min(max(p.channels - c, 0), kWide<T>) : 0;
+    __device__ __forceinline__ Channels(const ScanArgs<T>& p, int slab) {
+        c = (slab * p.lanes + static_cast<int>(threadIdx.x) % p.lanes) * N;
+        count = min(max(p.channels - c, 0), N);
         row_step = p.order.reverse ? -1 : 1;
     }
 
@@ -277,59 +278,71 @@ template <typename T, bool Whole, bool Backward> struct Walk {
     }
 
     // to: the thread's first channel in the row
-    __device__ __forceinline__ void store(T* to, const Row<T>& value) const {
-        Stored<T> raw;
-        if constexpr (sizeof(T) == 2) {
+    __device__ __forceinline__ void store(T* to, const Row<N>& value) const {
+        Stored<T, N> raw;
 #pragma unroll
-            for (int i = 0; i < Row<T>::kPairs; ++i) {
+        for (int i = 0; i < N / 2; ++i) {
+            if constexpr (sizeof(T) == 2) {
                 const __half2 h = __floats2half2_rn(value.v[i].x, value.v[i].y);
                 raw.v[2 * i] = __low2half(h);
                 raw.v[2 * i + 1] = __high2half(h);
+            } else {
+                raw.v[2 * i] = value.v[i].x;
+                raw.v[2 * i + 1] = value.v[i].y;
             }
-        } else {
-            raw.v[0] = value.v[0].x;
-            raw.v[1] = value.v[0].y;
         }
-        if constexpr (Whole) {
-            *reinterpret_cast<Stored<T>*>(to) = raw;
-        } else {
 #pragma unroll
-            for (int i = 0; i < kWide<T>; ++i) {
-                if (i < count) {
-                    to[i] = raw.v[i];
-                }
+        for (int i = 0; i < N; i += kMoveChannels) {
+            if (kMove == kBytes || i < count) {
+                using Part = Stored<T, kMoveChannels>;
+                *reinterpret_cast<Part*>(to + i) = reinterpret_cast<const Part&>(raw.v[i]);
             }
         }
     }
 
     // Row `row` of a float array [..][channels], or zeros without one.
-    __device__ __forceinline__ Row<T> state(const float* from, long long row, int channels) const {
-        Row<T> out = Row<T>::filled(0.0f);
+    __device__ __forceinline__ Row<N> state(const float* from, long long row, int channels) const {
+        Row<N> out = Row<N>::filled(0.0f);
         if (from != nullptr) {
             from += row * channels + c;
+            if (quads(from, channels)) {
 #pragma unroll
-            for (int i = 0; i < kWide<T>; ++i) {
-                if (Whole || i < count) {
-                    out.set(i, from[i]);
+                for (int i = 0; i + 3 < N; i += 4) {
+                    const float4 v = *reinterpret_cast<const float4*>(from + i);
+                    out.set(i, v.x);
+                    out.set(i + 1, v.y);
+                    out.set(i + 2, v.z);
+                    out.set(i + 3, v.w);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    if (i < count) {
+                        out.set(i, from[i]);
+                    }
                 }
             }
         }
         return out;
     }
 
-    __device__ __forceinline__ void store_state(float* to, long long row, int channels, const Row<T>& value) const {
+    // the thread's channels are whole quads of floats there
+    static __device__ __forceinline__ bool quads(const float* at, int channels) {
+        return kMove == kBytes && N % 4 == 0 && channels % 4 == 0 && reinterpret_cast<uintptr_t>(at) % 16 == 0;
+    }
+
+    __device__ __forceinline__ void store_state(float* to, long long row, int channels, const Row<N>& value) const {
         if (to != nullptr) {
             to += row * channels + c;
-            if constexpr (Whole) {
-                Pack<float, kWide<T>> out;
+            if (quads(to, channels)) {
 #pragma unroll
-                for (int i = 0; i < kWide<T>; ++i) {
-                    out.v[i] = value.get(i);
+                for (int i = 0; i + 3 < N; i += 4) {
+                    *reinterpret_cast<float4*>(to + i) =
+                        make_float4(value.get(i), value.get(i + 1), value.get(i + 2), value.get(i + 3));
                 }
-                store_pack<float, kWide<T>>(to, out);
             } else {
 #pragma unroll
-                for (int i = 0; i < kWide<T>; ++i) {
+                for (int i = 0; i < N; ++i) {
                     if (i < count) {
                         to[i] = value.get(i);
                     }
@@ -337,41 +350,61 @@ template <typename T, bool Whole, bool Backward> struct Walk {
             }
         }
     }
+
+    // The state that reaches the tile number `place` of the chain.
+    __device__ __forceinline__ Row<N> reaching(const ScanArgs<T>& p, int place) const {
+        Row<N> out = Row<N>::filled(0.0f);
+        if (p.maps != nullptr) {
+            const int group = place / p.per_group;
+            const float* state = p.states == nullptr ? nullptr : p.states + static_cast<size_t>(group) * p.channels + c;
+            const float2* map = p.maps + static_cast<size_t>(place) * p.channels + c;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                if (i < count) {
+                    out.set(i, apply(map[i], state == nullptr ? 0.0f : state[i]));
+                }
+            }
+        }
+        return out;
+    }
 };
 
 // Rows on their way from the arrays to a thread: a ring of stages in shared memory, each with
-// Rows rows of every array, filled by asynchronous copies of eight bytes. A thread copies what it
-// reads itself, so nothing is synchronised, and the bytes in flight (the memory needs some 50 KB
-// of them per SM) cost no registers.
-template <typename T, bool Whole, int Arrays, int Rows, int Stages> struct Ring {
-    static constexpr int kBytes = Stages * Arrays * Rows * kThreads * 8;
+// Rows rows of every array, filled by asynchronous copies. A thread copies what it reads itself,
+// so nothing is synchronised, and the bytes in flight (the memory needs some 50 KB of them per
+// SM) cost no registers.
+template <typename T, int N, int Granule, int Arrays, int Rows, int Stages> struct Ring {
+    using Lanes = Channels<T, N, Granule>;
+    static constexpr int kBytes = Stages * Arrays * Rows * kThreads * Lanes::kBytes;
 
-    __device__ __forceinline__ Stored<T>* slot(int stage, int array, int row) const {
+    __device__ __forceinline__ Stored<T, N>* slot(int stage, int array, int row) const {
         extern __shared__ __align__(16) unsigned char ring[];
-        return reinterpret_cast<Stored<T>*>(ring) + ((stage * Arrays + array) * Rows + row) * kThreads + threadIdx.x;
+        return reinterpret_cast<Stored<T, N>*>(ring) + ((stage * Arrays + array) * Rows + row) * kThreads + threadIdx.x;
     }
 
-    // `rows` more rows, at most Rows, from `at` on, which moves on to the row behind them; zeros
-    // for rows and channels that do not exist.
-    template <typename W>
-    __device__ __forceinline__ void fetch(const W& walk, int stage, int array, const T*& at, long long step, int rows) const {
-        if (Whole && rows >= Rows) {
-            const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot(stage, array, 0)));
+    // `rows` more rows, at most Rows, from `at` on, which moves on to the row behind them; what
+    // lies behind the last row or channel stays undefined.
+    __device__ __forceinline__ void fetch(const Lanes& lanes, int stage, int array, const T*& at, long long step, int rows) const {
+        const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(slot(stage, array, 0)));
 #pragma unroll
-            for (int r = 0; r < Rows; ++r) {
-                asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(to + r * kThreads * 8), "l"(at) : "memory");
-                at += step;
-            }
-        } else {
-            for (int r = 0; r < Rows; ++r) {
-                Stored<T> raw;
+        for (int r = 0; r < Rows; ++r) {
+            if (rows >= Rows || r < rows) {
 #pragma unroll
-                for (int i = 0; i < kWide<T>; ++i) {
-                    raw.v[i] = r < rows && i < walk.count ? at[i] : narrow<T>(0.0f);
+                for (int i = 0; i < N; i += Lanes::kMoveChannels) {
+                    if (Lanes::kMove == Lanes::kBytes || i < lanes.count) {
+                        const uint32_t target = to + r * kThreads * Lanes::kBytes + i * static_cast<int>(sizeof(T));
+                        if constexpr (Granule == 0) {
+                            slot(stage, array, r)->v[i] = at[i];
+                        } else if constexpr (Lanes::kMove == 16) {
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(target), "l"(at + i) : "memory");
+                        } else {
+                            asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(target), "l"(at + i),
+                                         "n"(Lanes::kMove) : "memory");
+                        }
+                    }
                 }
-                *slot(stage, array, r) = raw;
-                at += step;
             }
+            at += step;
         }
     }
 
@@ -379,63 +412,50 @@ template <typename T, bool Whole, int Arrays, int Rows, int Stages> struct Ring 
     __device__ __forceinline__ void commit() const { asm volatile("cp.async.commit_group;" ::: "memory"); }
     // the oldest stage is there; the ones behind it may still be on their way
     __device__ __forceinline__ void wait() const { asm volatile("cp.async.wait_group %0;" ::"n"(Stages - 2) : "memory"); }
+    __device__ __forceinline__ void drain() const { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
-    __device__ __forceinline__ Row<T> row(int stage, int array, int r) const { return Row<T>::from(*slot(stage, array, r)); }
+    __device__ __forceinline__ Row<N> row(int stage, int array, int r) const { return Row<N>::from(*slot(stage, array, r)); }
 };
 
 // Maps of the tiles of a group -> the maps before each tile in the group, and the group's map.
-template <typename T, typename W>
+// Takes the ring's memory.
+template <typename T, int N>
 __device__ __forceinline__ void share_maps(
-    const ScanArgs<T>& p, const W& walk, bool cut, const Row<T>& product, const Row<T>& sum
+    const ScanArgs<T>& p, int place, int c, int count, bool cut, const Row<N>& product, const Row<N>& sum
 ) {
-    constexpr int N = kWide<T>;
-    __shared__ float2 maps[N * kThreads];   // [tiles of the group][N * lanes]
+    extern __shared__ __align__(16) unsigned char ring[];
+    float2* maps = reinterpret_cast<float2*>(ring);   // [tiles of the group][N * lanes]
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         maps[N * threadIdx.x + i] = make_float2(cut ? kReset : product.get(i), sum.get(i));
     }
     __syncthreads();
-    const int width = N * p.lanes, tiles = kThreads / p.lanes;
+    const int width = N * p.lanes;
     if (static_cast<int>(threadIdx.x) < width) {
         float2 all = make_float2(1.0f, 0.0f);
-#pragma unroll 4
-        for (int k = 0; k < tiles; ++k) {
+#pragma unroll 8
+        for (int k = 0; k < p.per_group; ++k) {
             const float2 own = maps[k * width + threadIdx.x];
             maps[k * width + threadIdx.x] = all;
             all = compose(all, own);
         }
         const int group = blockIdx.x / p.slabs;
-        const int c = (blockIdx.x - group * p.slabs) * width + threadIdx.x;
-        if (c < p.channels) {
-            p.groups[static_cast<size_t>(group) * p.channels + c] = all;
+        const int channel = (blockIdx.x - group * p.slabs) * width + threadIdx.x;
+        if (channel < p.channels) {
+            p.groups[static_cast<size_t>(group) * p.channels + channel] = all;
         }
     }
     __syncthreads();
-    float2* to = p.maps + static_cast<size_t>(walk.place) * p.channels + walk.c;
+    if (place < p.tiles) {
+        float2* to = p.maps + static_cast<size_t>(place) * p.channels + c;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (i < walk.count) {
-            to[i] = maps[N * threadIdx.x + i];
-        }
-    }
-}
-
-// The state that reaches the thread's tile.
-template <typename T, typename W>
-__device__ __forceinline__ Row<T> reaching_state(const ScanArgs<T>& p, const W& walk, int block) {
-    Row<T> out = Row<T>::filled(0.0f);
-    if (p.maps != nullptr) {
-        const int group = block / p.slabs;
-        const float* state = p.states == nullptr ? nullptr : p.states + static_cast<size_t>(group) * p.channels + walk.c;
-        const float2* map = p.maps + static_cast<size_t>(walk.place) * p.channels + walk.c;
-#pragma unroll
-        for (int i = 0; i < kWide<T>; ++i) {
-            if (i < walk.count) {
-                out.set(i, apply(map[i], state == nullptr ? 0.0f : state[i]));
+        for (int i = 0; i < N; ++i) {
+            if (i < count) {
+                to[i] = maps[N * threadIdx.x + i];
             }
         }
     }
-    return out;
 }
 
 template <bool Value> struct Flag {
@@ -444,40 +464,41 @@ template <bool Value> struct Flag {
 
 // One row of the recurrence, as h = x + a (h - x): the weights of h and x add up to one whatever
 // the rounding of a, so a long memory does not gather it.
-template <typename T>
-__device__ __forceinline__ void advance(Row<T>& h, const Row<T>& a, const Row<T>& x) {
+template <int N> __device__ __forceinline__ void advance(Row<N>& h, const Row<N>& a, const Row<N>& x) {
 #pragma unroll
-    for (int i = 0; i < Row<T>::kPairs; ++i) {
+    for (int i = 0; i < Row<N>::kPairs; ++i) {
         h.v[i] = fma(a.v[i], minus(h.v[i], x.v[i]), x.v[i]);
     }
 }
 
-template <typename T> __device__ __forceinline__ Row<T> gates(const Row<T>& z) {
-    Row<T> a;
+template <int N> __device__ __forceinline__ Row<N> gates(const Row<N>& z) {
+    Row<N> a;
 #pragma unroll
-    for (int i = 0; i < Row<T>::kPairs; ++i) {
+    for (int i = 0; i < Row<N>::kPairs; ++i) {
         a.v[i] = sigmoid_from(exp_minus(z.v[i]));
     }
     return a;
 }
 
-constexpr int kRingRows = 4, kRingStages = 3;
+constexpr int kRingRows = 2, kRingStages = 4;
 
-template <typename T, bool Whole>
-__global__ void __launch_bounds__(kThreads, 4) recurrence_maps_kernel(ScanArgs<T> p) {
-    constexpr int R = kRingRows, S = kRingStages;
-    const Walk<T, Whole, false> walk(p, blockIdx.x);
-    const Ring<T, Whole, 2, R, S> ring;
-    Row<T> prod = Row<T>::filled(1.0f), h = Row<T>::filled(0.0f);
+template <typename T, int Granule>
+__global__ void __launch_bounds__(kThreads, 3) recurrence_maps_kernel(ScanArgs<T> p) {
+    constexpr int N = kMapBytes / static_cast<int>(sizeof(T)), R = kRingRows, S = kRingStages;
+    const int group = blockIdx.x / p.slabs;
+    const int place = group * p.per_group + static_cast<int>(threadIdx.x) / p.lanes;
+    const Channels<T, N, Granule> lanes(p, blockIdx.x - group * p.slabs);
+    const Ring<T, N, Granule, 2, R, S> ring;
+    Row<N> prod = Row<N>::filled(1.0f), h = Row<N>::filled(0.0f);
     bool cut = false;
-    if (walk.count > 0) {
-        const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
-        const T* from = walk.row(p.x, p.x_stride, p.order, first);
-        const T* gates_from = walk.row(p.z, p.z_stride, p.order, first);
+    if (place < p.tiles && lanes.count > 0) {
+        const int first = place * kTileRows, end = min(first + kTileRows, p.order.rows);
+        const T* from = lanes.row(p.x, p.x_stride, p.order, first);
+        const T* gates_from = lanes.row(p.z, p.z_stride, p.order, first);
         const auto fetch = [&](int row, int stage) {
             if (row < end) {
-                ring.fetch(walk, stage, 0, from, walk.row_step * p.x_stride, end - row);
-                ring.fetch(walk, stage, 1, gates_from, walk.row_step * p.z_stride, end - row);
+                ring.fetch(lanes, stage, 0, from, lanes.row_step * p.x_stride, end - row);
+                ring.fetch(lanes, stage, 1, gates_from, lanes.row_step * p.z_stride, end - row);
             }
             ring.commit();
         };
@@ -497,19 +518,19 @@ __global__ void __launch_bounds__(kThreads, 4) recurrence_maps_kernel(ScanArgs<T
                 for (int r = 0; r < R; ++r) {
                     if (decltype(marked)::value && row + r < cursor.begin) {
                         cut = true;
-                        h = Row<T>::filled(0.0f);
+                        h = Row<N>::filled(0.0f);
                         continue;
                     }
                     if (decltype(marked)::value && row + r == cursor.begin) {
                         cut = true;
-                        h = walk.state(p.initial, p.order.sequence(cursor.j), p.channels);
+                        h = lanes.state(p.initial, p.order.sequence(cursor.j), p.channels);
                     }
-                    const Row<T> a = gates<T>(ring.row(stage, 1, r));
+                    const Row<N> a = gates(ring.row(stage, 1, r));
 #pragma unroll
-                    for (int i = 0; i < Row<T>::kPairs; ++i) {
+                    for (int i = 0; i < Row<N>::kPairs; ++i) {
                         prod.v[i] = prod.v[i] * a.v[i];
                     }
-                    advance<T>(h, a, ring.row(stage, 0, r));
+                    advance(h, a, ring.row(stage, 0, r));
                     if (decltype(marked)::value && row + r == cursor.end - 1) {
                         cursor.next(p.order);
                     }
@@ -523,27 +544,29 @@ __global__ void __launch_bounds__(kThreads, 4) recurrence_maps_kernel(ScanArgs<T
             stage = (stage + 1) % S;
         }
     }
-    share_maps<T>(p, walk, cut, prod, h);
+    share_maps(p, place, lanes.c, lanes.count, cut, prod, h);
 }
 
-template <typename T, bool Whole>
-__global__ void __launch_bounds__(kThreads, 4) recurrence_apply_kernel(ScanArgs<T> p) {
-    constexpr int R = kRingRows, S = kRingStages;
+template <typename T, int Granule>
+__global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<T> p) {
+    constexpr int N = kMapBytes / static_cast<int>(sizeof(T)), R = kRingRows, S = kRingStages;
     // the last tiles first: the maps kernel read them last
     const int block = gridDim.x - 1 - blockIdx.x;
-    const Walk<T, Whole, false> walk(p, block);
-    const Ring<T, Whole, 2, R, S> ring;
+    const int group = block / p.slabs;
+    const int place = group * p.per_group + static_cast<int>(threadIdx.x) / p.lanes;
+    const Channels<T, N, Granule> lanes(p, block - group * p.slabs);
+    const Ring<T, N, Granule, 2, R, S> ring;
     check_offsets(p.order, p.status);
-    if (walk.count == 0) {
+    if (place >= p.tiles || lanes.count == 0) {
         return;
     }
-    const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
-    const T* from = walk.row(p.x, p.x_stride, p.order, first);
-    const T* gates_from = walk.row(p.z, p.z_stride, p.order, first);
+    const int first = place * kTileRows, end = min(first + kTileRows, p.order.rows);
+    const T* from = lanes.row(p.x, p.x_stride, p.order, first);
+    const T* gates_from = lanes.row(p.z, p.z_stride, p.order, first);
     const auto fetch = [&](int row, int stage) {
         if (row < end) {
-            ring.fetch(walk, stage, 0, from, walk.row_step * p.x_stride, end - row);
-            ring.fetch(walk, stage, 1, gates_from, walk.row_step * p.z_stride, end - row);
+            ring.fetch(lanes, stage, 0, from, lanes.row_step * p.x_stride, end - row);
+            ring.fetch(lanes, stage, 1, gates_from, lanes.row_step * p.z_stride, end - row);
         }
         ring.commit();
     };
@@ -551,18 +574,18 @@ __global__ void __launch_bounds__(kThreads, 4) recurrence_apply_kernel(ScanArgs<
     for (int s = 0; s < S - 1; ++s) {
         fetch(first + s * R, s);
     }
-    Row<T> h = reaching_state<T>(p, walk, block);
+    Row<N> h = lanes.reaching(p, place);
     Cursor cursor;
     cursor.seek(p.order, first);
-    const long long down = walk.row_step * p.channels;
-    T* out = p.h + static_cast<long long>(p.order.row(first)) * p.channels + walk.c;
+    const long long down = lanes.row_step * p.channels;
+    T* out = p.h + static_cast<long long>(p.order.row(first)) * p.channels + lanes.c;
     int stage = 0;
 #pragma unroll 1
     for (int row = first; row < end; row += R) {
         ring.wait();
         fetch(row + (S - 1) * R, (stage + S - 1) % S);
         if (row % kCarryRows == 0) {
-            walk.store_state(p.carries, row / kCarryRows, p.channels, h);
+            lanes.store_state(p.carries, row / kCarryRows, p.channels, h);
         }
         const auto write = [&](auto marked) {
 #pragma unroll
@@ -571,16 +594,16 @@ __global__ void __launch_bounds__(kThreads, 4) recurrence_apply_kernel(ScanArgs<
                     break;
                 }
                 if (decltype(marked)::value && row + r == cursor.begin) {
-                    h = walk.state(p.initial, p.order.sequence(cursor.j), p.channels);
+                    h = lanes.state(p.initial, p.order.sequence(cursor.j), p.channels);
                 }
-                advance<T>(h, gates<T>(ring.row(stage, 1, r)), ring.row(stage, 0, r));
+                advance(h, gates(ring.row(stage, 1, r)), ring.row(stage, 0, r));
                 if (decltype(marked)::value && row + r < cursor.begin) {
-                    h = Row<T>::filled(0.0f);
+                    h = Row<N>::filled(0.0f);
                 }
-                walk.store(out, h);
+                lanes.store(out, h);
                 out += down;
                 if (decltype(marked)::value && row + r == cursor.end - 1) {
-                    walk.store_state(p.final, p.order.sequence(cursor.j), p.channels, h);
+                    lanes.store_state(p.final, p.order.sequence(cursor.j), p.channels, h);
                     cursor.next(p.order);
                 }
             }
@@ -597,21 +620,23 @@ __global__ void __launch_bounds__(kThreads, 4) recurrence_apply_kernel(ScanArgs<
 // e_t = a_t dh_t is what a row hands to the row before it: e_t = a_t e_{t+1} + a_t dy_t, a chain
 // of the same kind backwards in time. A tile's map needs no walk backwards: what it hands out is
 // the sum of its dy_t times the product of its gates up to t, as far as the first sequence's end.
-template <typename T, bool Whole>
-__global__ void __launch_bounds__(kThreads, 4) recurrence_flow_maps_kernel(ScanArgs<T> p) {
-    constexpr int R = kRingRows, S = kRingStages;
-    const Walk<T, Whole, true> walk(p, blockIdx.x);
-    const Ring<T, Whole, 2, R, S> ring;
-    Row<T> prod = Row<T>::filled(1.0f), e = Row<T>::filled(0.0f);
+template <typename T, int Granule>
+__global__ void __launch_bounds__(kThreads, 3) recurrence_flow_maps_kernel(ScanArgs<T> p) {
+    constexpr int N = kMapBytes / static_cast<int>(sizeof(T)), R = kRingRows, S = kRingStages;
+    const int group = blockIdx.x / p.slabs;
+    const int place = group * p.per_group + static_cast<int>(threadIdx.x) / p.lanes;
+    const Channels<T, N, Granule> lanes(p, blockIdx.x - group * p.slabs);
+    const Ring<T, N, Granule, 2, R, S> ring;
+    Row<N> prod = Row<N>::filled(1.0f), e = Row<N>::filled(0.0f);
     bool open = true;
-    if (walk.count > 0) {
-        const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
-        const T* from = walk.row(p.dy, p.dy_stride, p.order, first);
-        const T* gates_from = walk.row(p.z, p.z_stride, p.order, first);
+    if (place < p.tiles && lanes.count > 0) {
+        const int first = (p.tiles - 1 - place) * kTileRows, end = min(first + kTileRows, p.order.rows);
+        const T* from = lanes.row(p.dy, p.dy_stride, p.order, first);
+        const T* gates_from = lanes.row(p.z, p.z_stride, p.order, first);
         const auto fetch = [&](int row, int stage) {
             if (row < end) {
-                ring.fetch(walk, stage, 0, from, walk.row_step * p.dy_stride, end - row);
-                ring.fetch(walk, stage, 1, gates_from, walk.row_step * p.z_stride, end - row);
+                ring.fetch(lanes, stage, 0, from, lanes.row_step * p.dy_stride, end - row);
+                ring.fetch(lanes, stage, 1, gates_from, lanes.row_step * p.z_stride, end - row);
             }
             ring.commit();
         };
@@ -631,17 +656,17 @@ __global__ void __launch_bounds__(kThreads, 4) recurrence_flow_maps_kernel(ScanA
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     const bool ends = decltype(marked)::value && row + r == cursor.end - 1;
-                    const Row<T> a = gates<T>(ring.row(stage, 1, r));
-                    Row<T> up = ring.row(stage, 0, r);
+                    const Row<N> a = gates(ring.row(stage, 1, r));
+                    Row<N> up = ring.row(stage, 0, r);
                     if (ends) {
-                        const Row<T> more = walk.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
+                        const Row<N> more = lanes.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
 #pragma unroll
-                        for (int i = 0; i < Row<T>::kPairs; ++i) {
+                        for (int i = 0; i < Row<N>::kPairs; ++i) {
                             up.v[i] = up.v[i] + more.v[i];
                         }
                     }
 #pragma unroll
-                    for (int i = 0; i < Row<T>::kPairs; ++i) {
+                    for (int i = 0; i < Row<N>::kPairs; ++i) {
                         prod.v[i] = prod.v[i] * a.v[i];
                         e.v[i] = fma(prod.v[i], up.v[i], e.v[i]);
                     }
@@ -658,43 +683,47 @@ __global__ void __launch_bounds__(kThreads, 4) recurrence_flow_maps_kernel(ScanA
             }
             stage = (stage + 1) % S;
         }
+        ring.drain();   // of an early end
     }
-    share_maps<T>(p, walk, !open, prod, e);
+    share_maps(p, place, lanes.c, lanes.count, !open, prod, e);
 }
 
 // Batches of rows from the last to the first. With q_t = a_t (h_{t-1} - x_t): h_t = x_t + q_t,
 // and dz_t = dx_t q_t.
-template <typename T, bool Whole>
+template <typename T, int Granule>
 __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanArgs<T> p) {
-    constexpr int R = kCarryRows, P = Row<T>::kPairs;
-    const int block = gridDim.x - 1 - blockIdx.x;
-    const Walk<T, Whole, true> walk(p, block);
-    const Ring<T, Whole, 3, R, 2> ring;
-    if (walk.count == 0) {
+    constexpr int N = kGradientBytes / static_cast<int>(sizeof(T)), R = kCarryRows, P = Row<N>::kPairs;
+    // time forwards, so the tiles that the maps kernel read last come first
+    const int spans = (p.tiles + kGradientTiles - 1) / kGradientTiles, per_block = kThreads / p.lanes;
+    const int span = static_cast<int>(blockIdx.x) / p.slabs * per_block + static_cast<int>(threadIdx.x) / p.lanes;
+    const Channels<T, N, Granule> lanes(p, blockIdx.x % p.slabs);
+    const Ring<T, N, Granule, 3, R, 2> ring;
+    if (span >= spans || lanes.count == 0) {
         return;
     }
-    const int first = walk.tile * kTileRows, end = min(first + kTileRows, p.order.rows);
+    constexpr int kSpanRows = kGradientTiles * kTileRows;
+    const int first = span * kSpanRows, end = min(first + kSpanRows, p.order.rows);
     const auto fetch = [&](int row, int stage) {
         if (row >= first) {
-            const T* x = walk.row(p.x, p.x_stride, p.order, row);
-            const T* z = walk.row(p.z, p.z_stride, p.order, row);
-            const T* dy = walk.row(p.dy, p.dy_stride, p.order, row);
-            ring.fetch(walk, stage, 0, x, walk.row_step * p.x_stride, end - row);
-            ring.fetch(walk, stage, 1, z, walk.row_step * p.z_stride, end - row);
-            ring.fetch(walk, stage, 2, dy, walk.row_step * p.dy_stride, end - row);
+            const T* x = lanes.row(p.x, p.x_stride, p.order, row);
+            const T* z = lanes.row(p.z, p.z_stride, p.order, row);
+            const T* dy = lanes.row(p.dy, p.dy_stride, p.order, row);
+            ring.fetch(lanes, stage, 0, x, lanes.row_step * p.x_stride, end - row);
+            ring.fetch(lanes, stage, 1, z, lanes.row_step * p.z_stride, end - row);
+            ring.fetch(lanes, stage, 2, dy, lanes.row_step * p.dy_stride, end - row);
         }
         ring.commit();
     };
     const int last = first + (end - 1 - first) / R * R;
     fetch(last, 0);
-    Row<T> e = reaching_state<T>(p, walk, block);
+    Row<N> e = lanes.reaching(p, p.tiles - 1 - min(span * kGradientTiles + kGradientTiles - 1, p.tiles - 1));
     Cursor cursor;
     cursor.seek(p.order, last);
-    const long long down = walk.row_step * p.channels;
+    const long long down = lanes.row_step * p.channels;
     int stage = 0;
 #pragma unroll 1
     for (int row = last; row >= first; row -= R) {
-        Row<T> h = walk.state(p.carries, row / R, p.channels);
+        Row<N> h = lanes.state(p.carries, row / R, p.channels);
         // from the sequence of the batch behind, or the one after it, back to the first that ends
         // behind this batch's first row
         while (cursor.begin > row) {
@@ -720,15 +749,15 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
         }
         ring.wait();
         fetch(row - R, stage ^ 1);
-        const long long at0 = static_cast<long long>(p.order.row(row)) * p.channels + walk.c;
+        const long long at0 = static_cast<long long>(p.order.row(row)) * p.channels + lanes.c;
         const auto differentiate = [&](auto marked) {
-            Row<T> odds[R], q[R];
+            Row<N> odds[R], q[R];
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 if (decltype(marked)::value && (heads >> r & 1u)) {
-                    h = walk.state(p.initial, p.order.sequence(cursor.j), p.channels);
+                    h = lanes.state(p.initial, p.order.sequence(cursor.j), p.channels);
                 }
-                const Row<T> zr = ring.row(stage, 1, r), xr = ring.row(stage, 0, r);
+                const Row<N> zr = ring.row(stage, 1, r), xr = ring.row(stage, 0, r);
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     odds[r].v[i] = exp_minus({max_or_nan(zr.v[i].x, kLowestGate), max_or_nan(zr.v[i].y, kLowestGate)});
@@ -743,10 +772,10 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
             for (int r = R - 1; r >= 0; --r) {
                 if (decltype(marked)::value && (tails >> r & 1u)) {
                     cursor.back(p.order);
-                    e = walk.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
+                    e = lanes.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
                 }
-                const Row<T> up = ring.row(stage, 2, r);
-                Row<T> dx, dz;
+                const Row<N> up = ring.row(stage, 2, r);
+                Row<N> dx, dz;
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     e.v[i] = sigmoid_from(odds[r].v[i]) * (up.v[i] + e.v[i]);
@@ -754,14 +783,14 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
                     dz.v[i] = dx.v[i] * q[r].v[i];
                 }
                 if (decltype(marked)::value && (dead >> r & 1u)) {
-                    dx = dz = e = Row<T>::filled(0.0f);
+                    dx = dz = e = Row<N>::filled(0.0f);
                 }
                 if (!decltype(marked)::value || row + r < end) {
-                    walk.store(p.dx + at0 + r * down, dx);
-                    walk.store(p.dz + at0 + r * down, dz);
+                    lanes.store(p.dx + at0 + r * down, dx);
+                    lanes.store(p.dz + at0 + r * down, dz);
                 }
                 if (decltype(marked)::value && (heads >> r & 1u)) {
-                    walk.store_state(p.dinitial, p.order.sequence(cursor.j), p.channels, e);
+                    lanes.store_state(p.dinitial, p.order.sequence(cursor.j), p.channels, e);
                 }
             }
         };
@@ -847,11 +876,11 @@ constexpr int kMaxRows = 0x7fffffff - kTileRows;   // row numbers of the last ti
 
 inline int tiles_of(long long rows) { return static_cast<int>((rows + kTileRows - 1) / kTileRows); }
 
-// Threads across a slab for `vectors` of eight bytes: 16, a 128-byte line, or fewer where that
-// leaves fewer of them without a channel.
-inline int slab_lanes(int vectors) {
-    int best = 16;
-    for (int lanes = 16; lanes >= 1; lanes >>= 1) {
+// Threads across a slab for so many threads' worth of channels: `most`, a 128-byte line, or fewer
+// where that leaves fewer of them without a channel.
+inline int slab_lanes(int vectors, int most) {
+    int best = most;
+    for (int lanes = most; lanes >= 1; lanes >>= 1) {
         if ((vectors + lanes - 1) / lanes * lanes < (vectors + best - 1) / best * best) {
             best = lanes;
         }
@@ -859,13 +888,16 @@ inline int slab_lanes(int vectors) {
     return best;
 }
 
+inline int vectors_of(int channels, int element, int bytes) { return (channels * element + bytes - 1) / bytes; }
+inline int map_lanes(int channels, int element) { return slab_lanes(vectors_of(channels, element, kMapBytes), 128 / kMapBytes); }
+
 struct ScanBytes {
     size_t maps, groups, states, total;
 };
 
-inline ScanBytes scan_bytes(long long rows, int channels, int wide) {
+inline ScanBytes scan_bytes(long long rows, int channels, int element) {
     ScanBytes b{};
-    const long long tiles = tiles_of(rows), per_group = kThreads / slab_lanes((channels + wide - 1) / wide);
+    const long long tiles = tiles_of(rows), per_group = kThreads / map_lanes(channels, element);
     const long long groups = (tiles + per_group - 1) / per_group;
     b.maps = align_up(sizeof(float2) * channels * tiles);
     b.groups = align_up(sizeof(float2) * channels * groups);
@@ -874,43 +906,44 @@ inline ScanBytes scan_bytes(long long rows, int channels, int wide) {
     return b;
 }
 
-template <typename T, bool Whole, bool Backward>
-int launch_scan(ScanArgs<T> p, void* workspace, size_t bytes, cudaStream_t stream) {
-    p.tiles = tiles_of(p.order.rows);
-    const int vectors = (p.channels + kWide<T> - 1) / kWide<T>;
-    p.lanes = slab_lanes(vectors);
-    p.slabs = (vectors + p.lanes - 1) / p.lanes;
-    const int per_group = kThreads / p.lanes;
-    const int groups = (p.tiles + per_group - 1) / per_group;
-    const long long blocks = static_cast<long long>(groups) * p.slabs;
+template <typename Kernel, typename T>
+int launch_walk(Kernel kernel, int ring_bytes, long long blocks, const ScanArgs<T>& p, cudaStream_t stream) {
     LAT_REQUIRE(blocks <= 0x7fffffffLL, "the recurrence supports at most 2^31 blocks of tiles.");
-    const ScanBytes b = scan_bytes(p.order.rows, p.channels, kWide<T>);
+    LAT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_bytes));
+    kernel<<<static_cast<unsigned>(blocks), kThreads, ring_bytes, stream>>>(p);
+    LAT_LAUNCH_CHECK();
+    return LAT_OK;
+}
+
+template <typename T, int Granule, bool Backward>
+int launch_scan(ScanArgs<T> p, void* workspace, size_t bytes, cudaStream_t stream) {
+    constexpr int kElement = static_cast<int>(sizeof(T)), N = kMapBytes / kElement, M = kGradientBytes / kElement;
+    constexpr int kRing = Ring<T, N, Granule, 2, kRingRows, kRingStages>::kBytes;
+    static_assert(kRing >= static_cast<int>(sizeof(float2)) * N * kThreads, "the ring's memory holds a group's maps");
+    p.tiles = tiles_of(p.order.rows);
+    p.lanes = map_lanes(p.channels, kElement);
+    p.per_group = kThreads / p.lanes;
+    const int vectors = vectors_of(p.channels, kElement, kMapBytes);
+    p.slabs = (vectors + p.lanes - 1) / p.lanes;
+    const int groups = (p.tiles + p.per_group - 1) / p.per_group;
+    const long long blocks = static_cast<long long>(groups) * p.slabs;
+    const ScanBytes b = scan_bytes(p.order.rows, p.channels, kElement);
     if (workspace == nullptr || bytes < b.total) {
         return fail(LAT_WORKSPACE_TOO_SMALL, "recurrence workspace is too small.");
     }
-    const unsigned grid = static_cast<unsigned>(blocks);
-    constexpr int kRing = Ring<T, Whole, 2, kRingRows, kRingStages>::kBytes;
-    constexpr int kApplyRing = Backward ? Ring<T, Whole, 3, kCarryRows, 2>::kBytes : kRing;
-    const void *maps_kernel, *apply_kernel;
-    if constexpr (Backward) {
-        maps_kernel = reinterpret_cast<const void*>(recurrence_flow_maps_kernel<T, Whole>);
-        apply_kernel = reinterpret_cast<const void*>(recurrence_gradient_kernel<T, Whole>);
-    } else {
-        maps_kernel = reinterpret_cast<const void*>(recurrence_maps_kernel<T, Whole>);
-        apply_kernel = reinterpret_cast<const void*>(recurrence_apply_kernel<T, Whole>);
-    }
-    LAT_CUDA_CHECK(cudaFuncSetAttribute(maps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRing));
-    LAT_CUDA_CHECK(cudaFuncSetAttribute(apply_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kApplyRing));
     if (p.tiles > 1) {
         char* base = static_cast<char*>(workspace);
         p.maps = reinterpret_cast<float2*>(base);
         p.groups = reinterpret_cast<float2*>(base + b.maps);
+        int code;
         if constexpr (Backward) {
-            recurrence_flow_maps_kernel<T, Whole><<<grid, kThreads, kRing, stream>>>(p);
+            code = launch_walk(recurrence_flow_maps_kernel<T, Granule>, kRing, blocks, p, stream);
         } else {
-            recurrence_maps_kernel<T, Whole><<<grid, kThreads, kRing, stream>>>(p);
+            code = launch_walk(recurrence_maps_kernel<T, Granule>, kRing, blocks, p, stream);
         }
-        LAT_LAUNCH_CHECK();
+        if (code != LAT_OK) {
+            return code;
+        }
         if (groups > 1) {
             p.states = reinterpret_cast<float*>(base + b.maps + b.groups);
             recurrence_scan_kernel<<<(p.channels + kScanChannels - 1) / kScanChannels, kScanChannels * kScanParts, 0,
@@ -919,27 +952,45 @@ int launch_scan(ScanArgs<T> p, void* workspace, size_t bytes, cudaStream_t strea
         }
     }
     if constexpr (Backward) {
-        recurrence_gradient_kernel<T, Whole><<<grid, kThreads, kApplyRing, stream>>>(p);
+        const int wide = vectors_of(p.channels, kElement, kGradientBytes);
+        const int spans = (p.tiles + kGradientTiles - 1) / kGradientTiles;
+        p.lanes = slab_lanes(wide, 128 / kGradientBytes);
+        p.slabs = (wide + p.lanes - 1) / p.lanes;
+        const int per_block = kThreads / p.lanes;
+        return launch_walk(recurrence_gradient_kernel<T, Granule>, Ring<T, M, Granule, 3, kCarryRows, 2>::kBytes,
+                           static_cast<long long>((spans + per_block - 1) / per_block) * p.slabs, p, stream);
     } else {
-        recurrence_apply_kernel<T, Whole><<<grid, kThreads, kApplyRing, stream>>>(p);
+        return launch_walk(recurrence_apply_kernel<T, Granule>, kRing, blocks, p, stream);
     }
-    LAT_LAUNCH_CHECK();
-    return LAT_OK;
 }
 
 template <typename T, bool Backward>
 int run_scan(const ScanArgs<T>& p, void* workspace, size_t bytes, cudaStream_t stream) {
-    constexpr int N = kWide<T>;
-    bool whole = p.channels % N == 0 && p.x_stride % N == 0 && p.z_stride % N == 0 && aligned_to(p.x, 8) && aligned_to(p.z, 8) &&
-                 aligned_to(p.carries, sizeof(float) * N) && aligned_to(p.initial, sizeof(float) * N);
-    if (Backward) {
-        whole = whole && p.dy_stride % N == 0 && aligned_to(p.dy, 8) && aligned_to(p.dx, 8) && aligned_to(p.dz, 8) &&
-                aligned_to(p.dinitial, sizeof(float) * N) && aligned_to(p.dfinal, sizeof(float) * N);
-    } else {
-        whole = whole && aligned_to(p.h, 8) && aligned_to(p.final, sizeof(float) * N);
+    const auto fits = [&](int granule) {
+        const int n = granule / static_cast<int>(sizeof(T));
+        bool ok = p.channels % n == 0 && p.x_stride % n == 0 && p.z_stride % n == 0 && aligned_to(p.x, granule) &&
+                  aligned_to(p.z, granule);
+        if (Backward) {
+            ok = ok && p.dy_stride % n == 0 && aligned_to(p.dy, granule) && aligned_to(p.dx, granule) &&
+                 aligned_to(p.dz, granule);
+        } else {
+            ok = ok && aligned_to(p.h, granule);
+        }
+        return ok;
+    };
+    if (fits(16)) {
+        return launch_scan<T, 16, Backward>(p, workspace, bytes, stream);
     }
-    return whole ? launch_scan<T, true, Backward>(p, workspace, bytes, stream)
-                 : launch_scan<T, false, Backward>(p, workspace, bytes, stream);
+    if (fits(8)) {
+        return launch_scan<T, 8, Backward>(p, workspace, bytes, stream);
+    }
+    if (fits(4)) {
+        return launch_scan<T, 4, Backward>(p, workspace, bytes, stream);
+    }
+    if constexpr (sizeof(T) == 2) {
+        return launch_scan<T, 0, Backward>(p, workspace, bytes, stream);
+    }
+    return fail(LAT_INVALID_ARGUMENT, "float32 features must be aligned to four bytes.");
 }
 
 // What a sequence without rows hands on: initial -> final, dfinal -> dinitial.
@@ -1011,7 +1062,7 @@ size_t lat_recurrence_workspace_bytes(int32_t dtype, int32_t rows, int32_t chann
     if (rows <= 0 || channels <= 0) {
         return 256;
     }
-    return scan_bytes(rows, channels, dtype == LAT_F32 ? kWide<float> : kWide<__half>).total;
+    return scan_bytes(rows, channels, dtype == LAT_F32 ? 4 : 2).total;
 }
 
 int32_t lat_recurrence_carry_rows(int32_t rows) {
