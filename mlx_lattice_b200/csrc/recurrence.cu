@@ -8,12 +8,12 @@
 //   dx_t = (1 - a_t) dh_t,  dz_t = a_t (1 - a_t) dh_t (h_{t-1} - x_t),  dinitial = a_1 dh_1
 //
 // Both directions are scans over affine maps h -> A h + H, which compose associatively. The
-// rows are cut into tiles of 32; a thread walks a tile for 16 bytes of channels. Three kernels:
-//   maps:   the map (A, H) of every tile, and for a group of tiles (a block) the maps of the
-//           tiles before each one in the group and of the whole group
-//   scan:   the state that reaches every group, from the groups' maps
-//   apply:  the state that reaches a tile is its map within the group applied to the group's
-//           state; walk the tile again from there and write
+// rows are cut into tiles of 32. Three kernels:
+//   maps:   for a group of tiles (a block, 128 rows of 128 bytes) the map (A, H) of the group and,
+//           for every tile, of the tiles before it in the group
+//   scan:   for every group the map of the groups before it in its window of 64, and the state
+//           that reaches every window
+//   apply:  those three give the state that reaches a tile; walk the tile from there and write
 // Nothing waits for anything inside a kernel, and every sum has a fixed order: results are
 // bitwise repeatable.
 //
@@ -34,11 +34,16 @@ namespace lat {
 namespace {
 
 constexpr int kTileRows = 32;
-constexpr int kThreads = 256;
+constexpr int kPieceRows = 8;                 // of a tile, walked by one thread of the maps kernel
+constexpr int kPieces = kTileRows / kPieceRows;
+constexpr int kMapThreads = 128;              // of a block of the maps kernel
+constexpr int kThreads = 256;                 // of the others
+constexpr int kWindow = 64;                   // groups
 constexpr int kMapBytes = 16;                 // channels of a thread of the maps and apply kernels
 constexpr int kGradientBytes = 8;             // of the gradient kernel, which keeps twice as much of each
 constexpr int kGradientTiles = 2;             // that a thread of the gradient kernel walks through
 constexpr float kReset = -1.0f;
+constexpr int kScanChannels = 32;             // of a block of the scan kernel
 constexpr int kCarryRows = 8;                 // rows from one kept state to the next
 
 // later after earlier, as maps
@@ -131,12 +136,22 @@ __device__ __forceinline__ Pair sigmoid_from(Pair odds) {
 }
 __device__ __forceinline__ float sigmoid_gate(float z) { return reciprocal(1.0f + exp2_fast(z * kMinusLog2E)); }
 
-// Offsets that fall are reported; the threads of the grid look at them in turn.
-__device__ __forceinline__ void check_offsets(const Order& order, int32_t* status) {
+// What the sequences ask for beside their rows, by the threads of the grid in turn: one without
+// rows hands on what it was given (`from`, or zeros) to `to`; offsets that fall are reported.
+__device__ __forceinline__ void visit_sequences(
+    const Order& order, const float* from, float* to, int channels, int32_t* status
+) {
     const long long threads = static_cast<long long>(gridDim.x) * blockDim.x;
     for (long long j = blockIdx.x * static_cast<long long>(blockDim.x) + threadIdx.x; j < order.sequences; j += threads) {
+        const int begin = order.begin(static_cast<int>(j)), end = order.begin(static_cast<int>(j) + 1);
         if (__ldg(order.offsets + j + 1) < __ldg(order.offsets + j)) {
             raise_status(status, LAT_STATUS_BAD_INDEX);
+        }
+        if (to != nullptr && end <= begin) {
+            const size_t at = static_cast<size_t>(order.sequence(static_cast<int>(j))) * channels;
+            for (int c = 0; c < channels; ++c) {
+                to[at + c] = from != nullptr ? from[at + c] : 0.0f;
+            }
         }
     }
 }
@@ -158,16 +173,17 @@ struct Cursor {
         begin = end = 0x7fffffff;
     }
 
-    // the first sequence that ends behind row `first`
-    __device__ __forceinline__ void seek(const Order& order, int first) {
+    // The first sequence that ends behind row `first`. `lanes` threads of a warp (`mask`, this one
+    // is number `lane`) ask together, at as many places a step.
+    __device__ __forceinline__ void seek(const Order& order, int first, int lane, int lanes, unsigned mask) {
         int low = 0, high = order.sequences;
         while (low < high) {
-            const int mid = (low + high) >> 1;
-            if (order.begin(mid + 1) > first) {
-                high = mid;
-            } else {
-                low = mid + 1;
-            }
+            const int step = (high - low) / (lanes + 1) + 1, at = low + (lane + 1) * step - 1;
+            // the answers rise: the sequence lies behind the last place that says no
+            const unsigned no = __ballot_sync(mask, at < high && order.begin(at + 1) <= first) & mask;
+            const int count = __popc(no);
+            high = count == lanes ? high : min(high, low + (count + 1) * step - 1);
+            low += count * step;
         }
         j = low;
         settle(order);
@@ -209,8 +225,10 @@ template <typename T> struct ScanArgs {
     int tiles;
     const float* initial;   // [sequences][channels] or null
     float2* maps;           // [tiles][channels] of the tiles before in the group
-    float2* groups;         // [groups][channels]
-    float* states;          // [groups][channels] that reach the groups, or null: zero
+    float2* groups;         // [groups][channels] of each group, then of the groups before in the window
+    float2* windows;        // [windows][channels] of each window
+    float* states;          // [windows][channels] that reach the windows
+    int* arrived;           // [scan slabs] blocks of the scan kernel that are done
     float* carries;         // [batches][channels] or null: h before each batch of rows
     T* h;
     float* final;           // [sequences][channels] or null
@@ -265,12 +283,21 @@ template <typename T, int N, int Granule> struct Channels {
     static constexpr int kMove = Granule == 0 ? static_cast<int>(sizeof(T)) : Granule < kBytes ? Granule : kBytes;
     static constexpr int kMoveChannels = kMove / static_cast<int>(sizeof(T));
     int c, count;
+    int lane, live;       // this thread and how many of the tile's threads have channels
     long long row_step;   // from a row to the next one, in rows of an array
 
     __device__ __forceinline__ Channels(const ScanArgs<T>& p, int slab) {
-        c = (slab * p.lanes + static_cast<int>(threadIdx.x) % p.lanes) * N;
+        lane = static_cast<int>(threadIdx.x) % p.lanes;
+        c = (slab * p.lanes + lane) * N;
         count = min(max(p.channels - c, 0), N);
+        live = min(p.lanes, (p.channels - slab * p.lanes * N + N - 1) / N);
         row_step = p.order.reverse ? -1 : 1;
+    }
+
+    // All live threads of the tile, together.
+    __device__ __forceinline__ void seek(Cursor& cursor, const Order& order, int first) const {
+        const unsigned mask = (live == 32 ? 0xffffffffu : (1u << live) - 1u) << ((threadIdx.x & 31) - lane);
+        cursor.seek(order, first, lane, live, mask);
     }
 
     __device__ __forceinline__ const T* row(const T* from, long long stride, const Order& order, int row) const {
@@ -355,13 +382,14 @@ template <typename T, int N, int Granule> struct Channels {
     __device__ __forceinline__ Row<N> reaching(const ScanArgs<T>& p, int place) const {
         Row<N> out = Row<N>::filled(0.0f);
         if (p.maps != nullptr) {
-            const int group = place / p.per_group;
-            const float* state = p.states == nullptr ? nullptr : p.states + static_cast<size_t>(group) * p.channels + c;
+            const int group = place / p.per_group, window = group / kWindow;
+            const float* state = p.states + static_cast<size_t>(window) * p.channels + c;
+            const float2* before = p.groups + static_cast<size_t>(group) * p.channels + c;
             const float2* map = p.maps + static_cast<size_t>(place) * p.channels + c;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
                 if (i < count) {
-                    out.set(i, apply(map[i], state == nullptr ? 0.0f : state[i]));
+                    out.set(i, apply(map[i], apply(before[i], state[i])));
                 }
             }
         }
@@ -373,13 +401,13 @@ template <typename T, int N, int Granule> struct Channels {
 // Rows rows of every array, filled by asynchronous copies. A thread copies what it reads itself,
 // so nothing is synchronised, and the bytes in flight (the memory needs some 50 KB of them per
 // SM) cost no registers.
-template <typename T, int N, int Granule, int Arrays, int Rows, int Stages> struct Ring {
+template <typename T, int N, int Granule, int Arrays, int Rows, int Stages, int Threads = kThreads> struct Ring {
     using Lanes = Channels<T, N, Granule>;
-    static constexpr int kBytes = Stages * Arrays * Rows * kThreads * Lanes::kBytes;
+    static constexpr int kBytes = Stages * Arrays * Rows * Threads * Lanes::kBytes;
 
     __device__ __forceinline__ Stored<T, N>* slot(int stage, int array, int row) const {
         extern __shared__ __align__(16) unsigned char ring[];
-        return reinterpret_cast<Stored<T, N>*>(ring) + ((stage * Arrays + array) * Rows + row) * kThreads + threadIdx.x;
+        return reinterpret_cast<Stored<T, N>*>(ring) + ((stage * Arrays + array) * Rows + row) * Threads + threadIdx.x;
     }
 
     // `rows` more rows, at most Rows, from `at` on, which moves on to the row behind them; what
@@ -392,7 +420,7 @@ template <typename T, int N, int Granule, int Arrays, int Rows, int Stages> stru
 #pragma unroll
                 for (int i = 0; i < N; i += Lanes::kMoveChannels) {
                     if (Lanes::kMove == Lanes::kBytes || i < lanes.count) {
-                        const uint32_t target = to + r * kThreads * Lanes::kBytes + i * static_cast<int>(sizeof(T));
+                        const uint32_t target = to + r * Threads * Lanes::kBytes + i * static_cast<int>(sizeof(T));
                         if constexpr (Granule == 0) {
                             slot(stage, array, r)->v[i] = at[i];
                         } else if constexpr (Lanes::kMove == 16) {
@@ -417,50 +445,61 @@ template <typename T, int N, int Granule, int Arrays, int Rows, int Stages> stru
     __device__ __forceinline__ Row<N> row(int stage, int array, int r) const { return Row<N>::from(*slot(stage, array, r)); }
 };
 
-// Maps of the tiles of a group -> the maps before each tile in the group, and the group's map.
-// Takes the ring's memory.
+// Maps of the pieces of a group -> the maps before each tile in the group, and the group's map.
+// Takes the ring's memory. A thread composes N pieces of a channel, a run of them; the runs
+// before its own give it the rest.
 template <typename T, int N>
-__device__ __forceinline__ void share_maps(
-    const ScanArgs<T>& p, int place, int c, int count, bool cut, const Row<N>& product, const Row<N>& sum
-) {
+__device__ __forceinline__ void share_maps(const ScanArgs<T>& p, bool cut, const Row<N>& product, const Row<N>& sum) {
+    static_assert(N % kPieces == 0, "a run holds whole tiles");
     extern __shared__ __align__(16) unsigned char ring[];
-    float2* maps = reinterpret_cast<float2*>(ring);   // [tiles of the group][N * lanes]
+    float2* maps = reinterpret_cast<float2*>(ring);   // [pieces of the group][N * lanes]
+    __shared__ float2 runs[kMapThreads];                 // [runs][N * lanes]
+    const int thread = threadIdx.x, width = N * p.lanes;
+    const int run = thread / width, lane = thread % width;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        maps[N * threadIdx.x + i] = make_float2(cut ? kReset : product.get(i), sum.get(i));
+        maps[N * thread + i] = make_float2(cut ? kReset : product.get(i), sum.get(i));
     }
     __syncthreads();
-    const int width = N * p.lanes;
-    if (static_cast<int>(threadIdx.x) < width) {
-        float2 all = make_float2(1.0f, 0.0f);
-#pragma unroll 8
-        for (int k = 0; k < p.per_group; ++k) {
-            const float2 own = maps[k * width + threadIdx.x];
-            maps[k * width + threadIdx.x] = all;
-            all = compose(all, own);
-        }
-        const int group = blockIdx.x / p.slabs;
-        const int channel = (blockIdx.x - group * p.slabs) * width + threadIdx.x;
-        if (channel < p.channels) {
-            p.groups[static_cast<size_t>(group) * p.channels + channel] = all;
-        }
-    }
-    __syncthreads();
-    if (place < p.tiles) {
-        float2* to = p.maps + static_cast<size_t>(place) * p.channels + c;
+    float2 before[N / kPieces], all = make_float2(1.0f, 0.0f);   // each tile of the run
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-            if (i < count) {
-                to[i] = maps[N * threadIdx.x + i];
-            }
+    for (int k = 0; k < N; ++k) {
+        if (k % kPieces == 0) {
+            before[k / kPieces] = all;
         }
+        all = compose(all, maps[(run * N + k) * width + lane]);
+    }
+    runs[thread] = all;
+    __syncthreads();
+    const int group = blockIdx.x / p.slabs;
+    const int channel = (blockIdx.x - group * p.slabs) * width + lane;
+    if (channel >= p.channels) {
+        return;
+    }
+    float2 rest = make_float2(1.0f, 0.0f);
+    for (int k = 0; k < run; ++k) {
+        rest = compose(rest, runs[k * width + lane]);
+    }
+    const int place = group * p.per_group + run * (N / kPieces);
+#pragma unroll
+    for (int t = 0; t < N / kPieces; ++t) {
+        if (place + t < p.tiles) {
+            p.maps[static_cast<size_t>(place + t) * p.channels + channel] = compose(rest, before[t]);
+        }
+    }
+    if (run == kMapThreads / width - 1) {
+        p.groups[static_cast<size_t>(group) * p.channels + channel] = compose(rest, all);
     }
 }
 
 template <bool Value> struct Flag {
     static constexpr bool value = Value;
 };
+
+// One answer for the lanes of a warp that are here: where one of them needs the path with marked
+// rows all take it, instead of both paths one after the other.
+__device__ __forceinline__ bool all_here(bool value) { return __all_sync(__activemask(), value); }
 
 // One row of the recurrence, as h = x + a (h - x): the weights of h and x add up to one whatever
 // the rounding of a, so a long memory does not gather it.
@@ -480,83 +519,107 @@ template <int N> __device__ __forceinline__ Row<N> gates(const Row<N>& z) {
     return a;
 }
 
-constexpr int kRingRows = 2, kRingStages = 4;
-
-template <typename T, int Granule>
-__global__ void __launch_bounds__(kThreads, 3) recurrence_maps_kernel(ScanArgs<T> p) {
-    constexpr int N = kMapBytes / static_cast<int>(sizeof(T)), R = kRingRows, S = kRingStages;
+// A group's rows are fetched at once and lie together, so this kernel streams: a thread walks
+// eight of them.
+//
+// Backwards, e_t = a_t dh_t is what a row hands to the row before it: e_t = a_t e_{t+1} + a_t dy_t,
+// a chain of the same kind with dy in the place of x. A piece's map needs no walk backwards: what
+// it hands out is the sum of its dy_t times the product of its gates up to t, as far as the first
+// sequence's end.
+template <typename T, int Granule, bool Backward>
+__global__ void __launch_bounds__(kMapThreads, 6) recurrence_maps_kernel(ScanArgs<T> p) {
+    constexpr int N = kMapBytes / static_cast<int>(sizeof(T)), R = kPieceRows;
     const int group = blockIdx.x / p.slabs;
-    const int place = group * p.per_group + static_cast<int>(threadIdx.x) / p.lanes;
+    // pieces in the order of the chain
+    const int place = group * p.per_group * kPieces + static_cast<int>(threadIdx.x) / p.lanes;
+    const int piece = Backward ? p.tiles * kPieces - 1 - place : place;
     const Channels<T, N, Granule> lanes(p, blockIdx.x - group * p.slabs);
-    const Ring<T, N, Granule, 2, R, S> ring;
-    Row<N> prod = Row<N>::filled(1.0f), h = Row<N>::filled(0.0f);
-    bool cut = false;
-    if (place < p.tiles && lanes.count > 0) {
-        const int first = place * kTileRows, end = min(first + kTileRows, p.order.rows);
-        const T* from = lanes.row(p.x, p.x_stride, p.order, first);
-        const T* gates_from = lanes.row(p.z, p.z_stride, p.order, first);
-        const auto fetch = [&](int row, int stage) {
-            if (row < end) {
-                ring.fetch(lanes, stage, 0, from, lanes.row_step * p.x_stride, end - row);
-                ring.fetch(lanes, stage, 1, gates_from, lanes.row_step * p.z_stride, end - row);
-            }
-            ring.commit();
-        };
-#pragma unroll
-        for (int s = 0; s < S - 1; ++s) {
-            fetch(first + s * R, s);
+    const Ring<T, N, Granule, 2, R, 1, kMapThreads> ring;
+    if (blockIdx.x == 0) {
+        for (int i = threadIdx.x; i < (p.channels + kScanChannels - 1) / kScanChannels; i += kMapThreads) {
+            p.arrived[i] = 0;
         }
-        Cursor cursor;
-        cursor.seek(p.order, first);
-        int stage = 0;
-#pragma unroll 1
-        for (int row = first; row < end; row += R) {
-            ring.wait();
-            fetch(row + (S - 1) * R, (stage + S - 1) % S);
-            const auto scan = [&](auto marked) {
+    }
+    Row<N> prod = Row<N>::filled(1.0f), sum = Row<N>::filled(0.0f);
+    bool cut = false;
+    const int first = piece * R, rows = p.order.rows - first;
+    if (piece >= 0 && rows > 0 && lanes.count > 0) {
+        const T* from = Backward ? lanes.row(p.dy, p.dy_stride, p.order, first) : lanes.row(p.x, p.x_stride, p.order, first);
+        const T* gates_from = lanes.row(p.z, p.z_stride, p.order, first);
+        ring.fetch(lanes, 0, 0, from, lanes.row_step * (Backward ? p.dy_stride : p.x_stride), rows);
+        ring.fetch(lanes, 0, 1, gates_from, lanes.row_step * p.z_stride, rows);
+        ring.commit();
+        Cursor cursor;   // meanwhile
+        lanes.seek(cursor, p.order, first);
+        const bool covered = all_here(cursor.covers(first, R));
+        ring.drain();
+        const auto scan = [&](auto marked) {
+            constexpr bool kMarked = decltype(marked)::value;
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    if (decltype(marked)::value && row + r < cursor.begin) {
-                        cut = true;
-                        h = Row<N>::filled(0.0f);
+            for (int r = 0; r < R; ++r) {
+                if (kMarked && first + r < cursor.begin) {
+                    cut = true;
+                    if constexpr (Backward) {
+                        break;   // a row outside all sequences hands nothing out
+                    } else {
+                        sum = Row<N>::filled(0.0f);
                         continue;
                     }
-                    if (decltype(marked)::value && row + r == cursor.begin) {
-                        cut = true;
-                        h = lanes.state(p.initial, p.order.sequence(cursor.j), p.channels);
-                    }
-                    const Row<N> a = gates(ring.row(stage, 1, r));
+                }
+                const Row<N> a = gates(ring.row(0, 1, r));
+                Row<N> value = ring.row(0, 0, r);
+                const bool ends = kMarked && first + r == cursor.end - 1;
+                if (Backward && ends) {
+                    const Row<N> more = lanes.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
 #pragma unroll
                     for (int i = 0; i < Row<N>::kPairs; ++i) {
-                        prod.v[i] = prod.v[i] * a.v[i];
+                        value.v[i] = value.v[i] + more.v[i];
                     }
-                    advance(h, a, ring.row(stage, 0, r));
-                    if (decltype(marked)::value && row + r == cursor.end - 1) {
+                }
+                if (!Backward && kMarked && first + r == cursor.begin) {
+                    cut = true;
+                    sum = lanes.state(p.initial, p.order.sequence(cursor.j), p.channels);
+                }
+#pragma unroll
+                for (int i = 0; i < Row<N>::kPairs; ++i) {
+                    prod.v[i] = prod.v[i] * a.v[i];
+                    if constexpr (Backward) {
+                        sum.v[i] = fma(prod.v[i], value.v[i], sum.v[i]);
+                    }
+                }
+                if constexpr (!Backward) {
+                    advance(sum, a, value);
+                }
+                if (ends) {
+                    if constexpr (Backward) {
+                        cut = true;
+                        break;
+                    } else {
                         cursor.next(p.order);
                     }
                 }
-            };
-            if (cursor.covers(row, R)) {
-                scan(Flag<false>{});
-            } else {
-                scan(Flag<true>{});
             }
-            stage = (stage + 1) % S;
+        };
+        if (covered) {
+            scan(Flag<false>{});
+        } else {
+            scan(Flag<true>{});
         }
     }
-    share_maps(p, place, lanes.c, lanes.count, cut, prod, h);
+    share_maps(p, cut, prod, sum);
 }
+
+constexpr int kRingRows = 2, kRingStages = 4;
 
 template <typename T, int Granule>
 __global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<T> p) {
     constexpr int N = kMapBytes / static_cast<int>(sizeof(T)), R = kRingRows, S = kRingStages;
     // the last tiles first: the maps kernel read them last
     const int block = gridDim.x - 1 - blockIdx.x;
-    const int group = block / p.slabs;
-    const int place = group * p.per_group + static_cast<int>(threadIdx.x) / p.lanes;
-    const Channels<T, N, Granule> lanes(p, block - group * p.slabs);
+    const int place = block / p.slabs * (kThreads / p.lanes) + static_cast<int>(threadIdx.x) / p.lanes;
+    const Channels<T, N, Granule> lanes(p, block % p.slabs);
     const Ring<T, N, Granule, 2, R, S> ring;
-    check_offsets(p.order, p.status);
+    visit_sequences(p.order, p.initial, p.final, p.channels, p.status);
     if (place >= p.tiles || lanes.count == 0) {
         return;
     }
@@ -576,7 +639,7 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<
     }
     Row<N> h = lanes.reaching(p, place);
     Cursor cursor;
-    cursor.seek(p.order, first);
+    lanes.seek(cursor, p.order, first);
     const long long down = lanes.row_step * p.channels;
     T* out = p.h + static_cast<long long>(p.order.row(first)) * p.channels + lanes.c;
     int stage = 0;
@@ -608,84 +671,13 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<
                 }
             }
         };
-        if (cursor.covers(row, R)) {
+        if (all_here(cursor.covers(row, R))) {
             write(Flag<false>{});
         } else {
             write(Flag<true>{});
         }
         stage = (stage + 1) % S;
     }
-}
-
-// e_t = a_t dh_t is what a row hands to the row before it: e_t = a_t e_{t+1} + a_t dy_t, a chain
-// of the same kind backwards in time. A tile's map needs no walk backwards: what it hands out is
-// the sum of its dy_t times the product of its gates up to t, as far as the first sequence's end.
-template <typename T, int Granule>
-__global__ void __launch_bounds__(kThreads, 3) recurrence_flow_maps_kernel(ScanArgs<T> p) {
-    constexpr int N = kMapBytes / static_cast<int>(sizeof(T)), R = kRingRows, S = kRingStages;
-    const int group = blockIdx.x / p.slabs;
-    const int place = group * p.per_group + static_cast<int>(threadIdx.x) / p.lanes;
-    const Channels<T, N, Granule> lanes(p, blockIdx.x - group * p.slabs);
-    const Ring<T, N, Granule, 2, R, S> ring;
-    Row<N> prod = Row<N>::filled(1.0f), e = Row<N>::filled(0.0f);
-    bool open = true;
-    if (place < p.tiles && lanes.count > 0) {
-        const int first = (p.tiles - 1 - place) * kTileRows, end = min(first + kTileRows, p.order.rows);
-        const T* from = lanes.row(p.dy, p.dy_stride, p.order, first);
-        const T* gates_from = lanes.row(p.z, p.z_stride, p.order, first);
-        const auto fetch = [&](int row, int stage) {
-            if (row < end) {
-                ring.fetch(lanes, stage, 0, from, lanes.row_step * p.dy_stride, end - row);
-                ring.fetch(lanes, stage, 1, gates_from, lanes.row_step * p.z_stride, end - row);
-            }
-            ring.commit();
-        };
-#pragma unroll
-        for (int s = 0; s < S - 1; ++s) {
-            fetch(first + s * R, s);
-        }
-        Cursor cursor;
-        cursor.seek(p.order, first);
-        open = first >= cursor.begin;   // a row outside all sequences hands nothing out
-        int stage = 0;
-#pragma unroll 1
-        for (int row = first; open && row < end; row += R) {
-            ring.wait();
-            fetch(row + (S - 1) * R, (stage + S - 1) % S);
-            const auto scan = [&](auto marked) {
-#pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const bool ends = decltype(marked)::value && row + r == cursor.end - 1;
-                    const Row<N> a = gates(ring.row(stage, 1, r));
-                    Row<N> up = ring.row(stage, 0, r);
-                    if (ends) {
-                        const Row<N> more = lanes.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
-#pragma unroll
-                        for (int i = 0; i < Row<N>::kPairs; ++i) {
-                            up.v[i] = up.v[i] + more.v[i];
-                        }
-                    }
-#pragma unroll
-                    for (int i = 0; i < Row<N>::kPairs; ++i) {
-                        prod.v[i] = prod.v[i] * a.v[i];
-                        e.v[i] = fma(prod.v[i], up.v[i], e.v[i]);
-                    }
-                    if (ends) {
-                        open = false;
-                        break;
-                    }
-                }
-            };
-            if (cursor.covers(row, R)) {
-                scan(Flag<false>{});
-            } else {
-                scan(Flag<true>{});
-            }
-            stage = (stage + 1) % S;
-        }
-        ring.drain();   // of an early end
-    }
-    share_maps(p, place, lanes.c, lanes.count, !open, prod, e);
 }
 
 // Batches of rows from the last to the first. With q_t = a_t (h_{t-1} - x_t): h_t = x_t + q_t,
@@ -698,6 +690,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
     const int span = static_cast<int>(blockIdx.x) / p.slabs * per_block + static_cast<int>(threadIdx.x) / p.lanes;
     const Channels<T, N, Granule> lanes(p, blockIdx.x % p.slabs);
     const Ring<T, N, Granule, 3, R, 2> ring;
+    visit_sequences(p.order, p.dfinal, p.dinitial, p.channels, nullptr);
     if (span >= spans || lanes.count == 0) {
         return;
     }
@@ -718,7 +711,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
     fetch(last, 0);
     Row<N> e = lanes.reaching(p, p.tiles - 1 - min(span * kGradientTiles + kGradientTiles - 1, p.tiles - 1));
     Cursor cursor;
-    cursor.seek(p.order, last);
+    lanes.seek(cursor, p.order, last);
     const long long down = lanes.row_step * p.channels;
     int stage = 0;
 #pragma unroll 1
@@ -733,7 +726,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
             }
             cursor = before;
         }
-        const bool covered = cursor.covers(row, R);
+        const bool covered = all_here(cursor.covers(row, R));
         // of the batch's rows: start a sequence, end one, lie outside all
         unsigned heads = 0, tails = 0, dead = 0;
         if (!covered) {
@@ -803,43 +796,87 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
     }
 }
 
-// From the groups' maps to the state that reaches each group: kScanChannels channels a block,
-// kScanParts threads a channel. A thread composes a run of groups, the threads of a channel scan
-// their maps, and each walks its run again.
-constexpr int kScanChannels = 8, kScanParts = 128;
+// A run of kRun maps of a channel by every warp of a block, kWindow by the block: each becomes
+// the map of those before it, and the map of all comes back to every thread.
+constexpr int kScanWarps = 8, kRun = kWindow / kScanWarps;
 
-__global__ void __launch_bounds__(kScanChannels * kScanParts) recurrence_scan_kernel(
-    const float2* groups, int count, int channels, float* states
-) {
-    __shared__ float2 maps[kScanParts][kScanChannels];
-    const int lane = threadIdx.x % kScanChannels, part = threadIdx.x / kScanChannels;
-    const int c = blockIdx.x * kScanChannels + lane;
-    const bool in = c < channels;
-    const int run = (count + kScanParts - 1) / kScanParts;
-    const int begin = min(part * run, count), end = min(begin + run, count);
-    float2 map = make_float2(1.0f, 0.0f);
-    if (in) {
-#pragma unroll 4
-        for (int g = begin; g < end; ++g) {
-            map = compose(map, groups[static_cast<size_t>(g) * channels + c]);
-        }
+__device__ __forceinline__ float2 scan_maps(float2 (&maps)[kRun], float2 (&shared)[kScanWarps][32]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float2 all = make_float2(1.0f, 0.0f);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        const float2 own = maps[i];
+        maps[i] = all;
+        all = compose(all, own);
     }
-    maps[part][lane] = map;
+    __syncthreads();   // a second call writes what the first one read
+    shared[warp][lane] = all;
     __syncthreads();
-    for (int d = 1; d < kScanParts; d <<= 1) {
-        const float2 before = part >= d ? maps[part - d][lane] : make_float2(1.0f, 0.0f);
-        __syncthreads();
-        map = compose(before, map);
-        maps[part][lane] = map;
-        __syncthreads();
+    float2 before = make_float2(1.0f, 0.0f), total = before;
+#pragma unroll
+    for (int w = 0; w < kScanWarps; ++w) {
+        before = w == warp ? total : before;
+        total = compose(total, shared[w][lane]);
     }
-    float h = part > 0 ? apply(maps[part - 1][lane], 0.0f) : 0.0f;
-    if (in) {
-#pragma unroll 4
-        for (int g = begin; g < end; ++g) {
-            states[static_cast<size_t>(g) * channels + c] = h;
-            h = apply(groups[static_cast<size_t>(g) * channels + c], h);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        maps[i] = compose(before, maps[i]);
+    }
+    return total;
+}
+
+// Block: a window of groups for 32 channels. The last block of these channels to be done goes on
+// to the states of the windows: which block that is does not change what it computes.
+__global__ void __launch_bounds__(32 * kScanWarps) recurrence_scan_kernel(
+    float2* groups, int count, int channels, float2* windows, float* states, int* arrived
+) {
+    __shared__ float2 shared[kScanWarps][32];
+    __shared__ bool last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c = blockIdx.y * 32 + lane;
+    const auto load = [&](const float2* from, int first, int end, float2 (&maps)[kRun]) {
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+            maps[i] = c < channels && first + i < end ? __ldcg(from + static_cast<size_t>(first + i) * channels + c)
+                                                      : make_float2(1.0f, 0.0f);
         }
+    };
+    float2 maps[kRun];
+    int first = blockIdx.x * kWindow + warp * kRun;
+    load(groups, first, count, maps);
+    const float2 total = scan_maps(maps, shared);
+#pragma unroll
+    for (int i = 0; i < kRun; ++i) {
+        if (c < channels && first + i < count) {
+            groups[static_cast<size_t>(first + i) * channels + c] = maps[i];
+        }
+    }
+    if (warp == 0 && c < channels) {
+        __stcg(windows + static_cast<size_t>(blockIdx.x) * channels + c, total);
+    }
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        last = atomicAdd(arrived + blockIdx.y, 1) == static_cast<int>(gridDim.x) - 1;
+    }
+    __syncthreads();
+    if (!last) {
+        return;
+    }
+    __threadfence();
+    const int windows_count = gridDim.x;
+    float h = 0.0f;
+    for (int base = 0; base < windows_count; base += kWindow) {
+        first = base + warp * kRun;
+        load(windows, first, windows_count, maps);
+        const float2 all = scan_maps(maps, shared);
+#pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+            if (c < channels && first + i < windows_count) {
+                states[static_cast<size_t>(first + i) * channels + c] = apply(maps[i], h);
+            }
+        }
+        h = apply(all, h);
     }
 }
 
@@ -876,41 +913,48 @@ constexpr int kMaxRows = 0x7fffffff - kTileRows;   // row numbers of the last ti
 
 inline int tiles_of(long long rows) { return static_cast<int>((rows + kTileRows - 1) / kTileRows); }
 
-// Threads across a slab for so many threads' worth of channels: `most`, a 128-byte line, or fewer
-// where that leaves fewer of them without a channel.
+// Threads across a slab for so many threads' worth of channels: `most`, a 128-byte line, or half
+// of them where that leaves fewer without a channel; for fewer channels the next power of two.
 inline int slab_lanes(int vectors, int most) {
-    int best = most;
-    for (int lanes = most; lanes >= 1; lanes >>= 1) {
-        if ((vectors + lanes - 1) / lanes * lanes < (vectors + best - 1) / best * best) {
-            best = lanes;
+    if (vectors < most) {
+        int lanes = 1;
+        while (lanes < vectors) {
+            lanes <<= 1;
         }
+        return lanes;
     }
-    return best;
+    const int half = most / 2;
+    return (vectors + half - 1) / half * half < (vectors + most - 1) / most * most ? half : most;
 }
 
 inline int vectors_of(int channels, int element, int bytes) { return (channels * element + bytes - 1) / bytes; }
 inline int map_lanes(int channels, int element) { return slab_lanes(vectors_of(channels, element, kMapBytes), 128 / kMapBytes); }
 
+// tiles of a group: a block of the maps kernel
+inline int group_tiles(int lanes) { return kMapThreads / lanes / kPieces; }
+
 struct ScanBytes {
-    size_t maps, groups, states, total;
+    size_t maps, groups, windows, states, total;
 };
 
 inline ScanBytes scan_bytes(long long rows, int channels, int element) {
     ScanBytes b{};
-    const long long tiles = tiles_of(rows), per_group = kThreads / map_lanes(channels, element);
-    const long long groups = (tiles + per_group - 1) / per_group;
+    const long long tiles = tiles_of(rows), per_group = group_tiles(map_lanes(channels, element));
+    const long long groups = (tiles + per_group - 1) / per_group, windows = (groups + kWindow - 1) / kWindow;
     b.maps = align_up(sizeof(float2) * channels * tiles);
     b.groups = align_up(sizeof(float2) * channels * groups);
-    b.states = align_up(sizeof(float) * channels * groups);
-    b.total = tiles <= 1 ? 256 : b.maps + b.groups + b.states;
+    b.windows = align_up(sizeof(float2) * channels * windows);
+    b.states = align_up(sizeof(float) * channels * windows);
+    const size_t arrived = align_up(sizeof(int) * ((channels + kScanChannels - 1) / kScanChannels));
+    b.total = tiles <= 1 ? 256 : b.maps + b.groups + b.windows + b.states + arrived;
     return b;
 }
 
 template <typename Kernel, typename T>
-int launch_walk(Kernel kernel, int ring_bytes, long long blocks, const ScanArgs<T>& p, cudaStream_t stream) {
+int launch_walk(Kernel kernel, int threads, int ring_bytes, long long blocks, const ScanArgs<T>& p, cudaStream_t stream) {
     LAT_REQUIRE(blocks <= 0x7fffffffLL, "the recurrence supports at most 2^31 blocks of tiles.");
     LAT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, ring_bytes));
-    kernel<<<static_cast<unsigned>(blocks), kThreads, ring_bytes, stream>>>(p);
+    kernel<<<static_cast<unsigned>(blocks), threads, ring_bytes, stream>>>(p);
     LAT_LAUNCH_CHECK();
     return LAT_OK;
 }
@@ -919,10 +963,10 @@ template <typename T, int Granule, bool Backward>
 int launch_scan(ScanArgs<T> p, void* workspace, size_t bytes, cudaStream_t stream) {
     constexpr int kElement = static_cast<int>(sizeof(T)), N = kMapBytes / kElement, M = kGradientBytes / kElement;
     constexpr int kRing = Ring<T, N, Granule, 2, kRingRows, kRingStages>::kBytes;
-    static_assert(kRing >= static_cast<int>(sizeof(float2)) * N * kThreads, "the ring's memory holds a group's maps");
+    constexpr int kMapsRing = Ring<T, N, Granule, 2, kPieceRows, 1, kMapThreads>::kBytes;
     p.tiles = tiles_of(p.order.rows);
     p.lanes = map_lanes(p.channels, kElement);
-    p.per_group = kThreads / p.lanes;
+    p.per_group = group_tiles(p.lanes);
     const int vectors = vectors_of(p.channels, kElement, kMapBytes);
     p.slabs = (vectors + p.lanes - 1) / p.lanes;
     const int groups = (p.tiles + p.per_group - 1) / p.per_group;
@@ -935,21 +979,19 @@ int launch_scan(ScanArgs<T> p, void* workspace, size_t bytes, cudaStream_t strea
         char* base = static_cast<char*>(workspace);
         p.maps = reinterpret_cast<float2*>(base);
         p.groups = reinterpret_cast<float2*>(base + b.maps);
-        int code;
-        if constexpr (Backward) {
-            code = launch_walk(recurrence_flow_maps_kernel<T, Granule>, kRing, blocks, p, stream);
-        } else {
-            code = launch_walk(recurrence_maps_kernel<T, Granule>, kRing, blocks, p, stream);
-        }
+        p.windows = reinterpret_cast<float2*>(base + b.maps + b.groups);
+        p.states = reinterpret_cast<float*>(base + b.maps + b.groups + b.windows);
+        p.arrived = reinterpret_cast<int*>(base + b.maps + b.groups + b.windows + b.states);
+        const int code =
+            launch_walk(recurrence_maps_kernel<T, Granule, Backward>, kMapThreads, kMapsRing, blocks, p, stream);
         if (code != LAT_OK) {
             return code;
         }
-        if (groups > 1) {
-            p.states = reinterpret_cast<float*>(base + b.maps + b.groups);
-            recurrence_scan_kernel<<<(p.channels + kScanChannels - 1) / kScanChannels, kScanChannels * kScanParts, 0,
-                                     stream>>>(p.groups, groups, p.channels, p.states);
-            LAT_LAUNCH_CHECK();
-        }
+        const dim3 scan_grid((groups + kWindow - 1) / kWindow, (p.channels + kScanChannels - 1) / kScanChannels);
+        LAT_REQUIRE(scan_grid.y <= 65535, "the recurrence supports at most two million channels.");
+        recurrence_scan_kernel<<<scan_grid, 32 * kScanWarps, 0, stream>>>(p.groups, groups, p.channels, p.windows,
+                                                                          p.states, p.arrived);
+        LAT_LAUNCH_CHECK();
     }
     if constexpr (Backward) {
         const int wide = vectors_of(p.channels, kElement, kGradientBytes);
@@ -957,10 +999,12 @@ int launch_scan(ScanArgs<T> p, void* workspace, size_t bytes, cudaStream_t strea
         p.lanes = slab_lanes(wide, 128 / kGradientBytes);
         p.slabs = (wide + p.lanes - 1) / p.lanes;
         const int per_block = kThreads / p.lanes;
-        return launch_walk(recurrence_gradient_kernel<T, Granule>, Ring<T, M, Granule, 3, kCarryRows, 2>::kBytes,
+        return launch_walk(recurrence_gradient_kernel<T, Granule>, kThreads, Ring<T, M, Granule, 3, kCarryRows, 2>::kBytes,
                            static_cast<long long>((spans + per_block - 1) / per_block) * p.slabs, p, stream);
     } else {
-        return launch_walk(recurrence_apply_kernel<T, Granule>, kRing, blocks, p, stream);
+        const int per_block = kThreads / p.lanes;
+        return launch_walk(recurrence_apply_kernel<T, Granule>, kThreads, kRing,
+                           static_cast<long long>((p.tiles + per_block - 1) / per_block) * p.slabs, p, stream);
     }
 }
 
@@ -993,7 +1037,7 @@ int run_scan(const ScanArgs<T>& p, void* workspace, size_t bytes, cudaStream_t s
     return fail(LAT_INVALID_ARGUMENT, "float32 features must be aligned to four bytes.");
 }
 
-// What a sequence without rows hands on: initial -> final, dfinal -> dinitial.
+// Without any rows: initial -> final, dfinal -> dinitial.
 inline int hand_over(const float* from, float* to, int sequences, int channels, cudaStream_t stream) {
     const size_t bytes = sizeof(float) * static_cast<size_t>(sequences) * channels;
     if (to == nullptr || bytes == 0) {
@@ -1081,9 +1125,8 @@ int lat_recurrence_forward(
     LAT_REQUIRE(sequences >= 0 && (sequences == 0 || offsets != nullptr),
                 "offsets must hold one int32 entry per sequence and one more.");
     cudaStream_t stream = as_stream(stream_ptr);
-    int code = hand_over(initial_state, final_state, sequences, channels, stream);
-    if (code != LAT_OK || rows == 0) {
-        return code;
+    if (rows == 0) {
+        return hand_over(initial_state, final_state, sequences, channels, stream);
     }
     LAT_REQUIRE(feats != nullptr && gate != nullptr && out != nullptr, "feats and gate must have shape (N, C).");
     LAT_REQUIRE(offsets != nullptr, "offsets must hold one int32 entry per sequence and one more.");
@@ -1109,9 +1152,8 @@ int lat_recurrence_backward(
     LAT_REQUIRE(sequences >= 0 && (sequences == 0 || offsets != nullptr),
                 "offsets must hold one int32 entry per sequence and one more.");
     cudaStream_t stream = as_stream(stream_ptr);
-    int code = hand_over(grad_final, grad_initial, sequences, channels, stream);
-    if (code != LAT_OK || rows == 0) {
-        return code;
+    if (rows == 0) {
+        return hand_over(grad_final, grad_initial, sequences, channels, stream);
     }
     LAT_REQUIRE(feats != nullptr && gate != nullptr && grad != nullptr && grad_feats != nullptr &&
                     grad_gate != nullptr && carries != nullptr,
