@@ -9,11 +9,12 @@
 // gradient: it draws the same words again. A dropped element is selected away, not multiplied
 // by zero, so an infinity or a NaN in a dropped place is gone.
 //
-// Bound by the memory: one read of x (and of the residual), one write of y. A thread takes 16
-// bytes: one counter for four floats, two for eight halves.
+// One read of x (and of the residual), one write of y. A thread takes 16 bytes: one counter for
+// four floats, two for eight halves.
 #include <algorithm>
 
 #include "common.cuh"
+#include "pairs.cuh"
 #include "vector_io.cuh"
 
 namespace lat {
@@ -22,102 +23,118 @@ namespace {
 
 constexpr int kThreads = 256;
 
+constexpr int kRounds = 10;
+
+// The keys of the rounds. They are the same for every element, so the host makes them; from a
+// seed on the device every thread makes them, for all its elements.
+struct Keys {
+    uint32_t k0[kRounds], k1[kRounds];
+};
+
+__host__ __device__ inline Keys round_keys(unsigned long long seed) {
+    Keys keys;
+    uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
+#pragma unroll
+    for (int round = 0; round < kRounds; ++round) {
+        keys.k0[round] = k0;
+        keys.k1[round] = k1;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
+    }
+    return keys;
+}
+
 struct Words {
     uint32_t w[4];
 };
 
-__device__ __forceinline__ Words philox(unsigned long long index, unsigned long long offset, unsigned long long seed) {
+__device__ __forceinline__ void multiply(uint32_t a, uint32_t b, uint32_t& low, uint32_t& high) {
+    asm("{\n.reg .b64 p;\nmul.wide.u32 p, %2, %3;\nmov.b64 {%0, %1}, p;\n}" : "=r"(low), "=r"(high) : "r"(a), "r"(b));
+}
+
+__device__ __forceinline__ Words philox(unsigned long long index, unsigned long long offset, const Keys& keys) {
     uint32_t c0 = static_cast<uint32_t>(index), c1 = static_cast<uint32_t>(index >> 32);
     uint32_t c2 = static_cast<uint32_t>(offset), c3 = static_cast<uint32_t>(offset >> 32);
-    uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
 #pragma unroll
-    for (int round = 0; round < 10; ++round) {
-        const unsigned long long a = static_cast<unsigned long long>(c0) * 0xD2511F53u;
-        const unsigned long long b = static_cast<unsigned long long>(c2) * 0xCD9E8D57u;
-        c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
-        c1 = static_cast<uint32_t>(b);
-        c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
-        c3 = static_cast<uint32_t>(a);
-        k0 += 0x9E3779B9u;
-        k1 += 0xBB67AE85u;
+    for (int round = 0; round < kRounds; ++round) {
+        uint32_t a_low, a_high, b_low, b_high;
+        multiply(c0, 0xD2511F53u, a_low, a_high);
+        multiply(c2, 0xCD9E8D57u, b_low, b_high);
+        c0 = b_high ^ c1 ^ keys.k0[round];
+        c1 = b_low;
+        c2 = a_high ^ c3 ^ keys.k1[round];
+        c3 = a_low;
     }
     return {{c0, c1, c2, c3}};
 }
 
-// V elements a thread, a multiple of four; the last ones of an odd total one by one.
-template <typename T, int V>
+// Element i of the words, kept or dropped, plus the residual.
+template <typename T, bool Residual>
+__device__ __forceinline__ float drop(float x, float add, uint32_t word, uint32_t threshold, float scale) {
+    const float kept = word >= threshold ? x * scale : 0.0f;
+    return Residual ? kept + add : kept;
+}
+
+// V elements a thread, a multiple of four; the last ones of an odd total one by one. Aligned:
+// V elements can be moved at once. What bounds it is the generator, 40 instructions for four
+// elements, a little above the memory for float16 and below it for float32.
+template <typename T, int V, bool Aligned, bool Residual, bool DeviceSeed>
 __global__ void __launch_bounds__(kThreads) dropout_kernel(
-    const T* x, const T* residual, long long total, uint32_t threshold, float scale, unsigned long long seed,
-    const unsigned long long* seed_device, unsigned long long offset, T* out
+    const T* x, const T* residual, long long total, uint32_t threshold, float scale, Keys keys,
+    const unsigned long long* seed, unsigned long long offset, T* out
 ) {
     const long long first = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) * V;
     if (first >= total) {
         return;
     }
-    if (seed_device != nullptr) {
-        seed = __ldg(seed_device);
-    }
     // the loads are on their way while the words are computed
-    const bool whole = first + V <= total;
+    const bool whole = Aligned && first + V <= total;
     Pack<T, V> in, add, y;
     if (whole) {
         in = load_pack<T, V>(x + first);
-        if (residual != nullptr) {
+        if (Residual) {
             add = load_pack<T, V>(residual + first);
         }
+    }
+    if (DeviceSeed) {
+        keys = round_keys(__ldg(seed));
     }
     Words words[V / 4];
 #pragma unroll
     for (int q = 0; q < V / 4; ++q) {
-        words[q] = philox(static_cast<unsigned long long>(first) / 4 + q, offset, seed);
+        words[q] = philox(static_cast<unsigned long long>(first) / 4 + q, offset, keys);
     }
     if (whole) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            float v = words[i / 4].w[i % 4] >= threshold ? in.get(i) * scale : 0.0f;
-            if (residual != nullptr) {
-                v += add.get(i);
-            }
-            y.set(i, v);
+        for (int i = 0; i < V; i += 2) {
+            const Pair v = get_pair(in, i / 2);
+            const Pair more = Residual ? get_pair(add, i / 2) : both(0.0f);
+            set_pair(y, i / 2, {drop<T, Residual>(v.x, more.x, words[i / 4].w[i % 4], threshold, scale),
+                                drop<T, Residual>(v.y, more.y, words[i / 4].w[i % 4 + 1], threshold, scale)});
         }
         store_pack<T, V>(out + first, y);
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             if (first + i < total) {
-                float v = words[i / 4].w[i % 4] >= threshold ? widen<T>(x[first + i]) * scale : 0.0f;
-                if (residual != nullptr) {
-                    v += widen<T>(residual[first + i]);
-                }
-                out[first + i] = narrow<T>(v);
+                out[first + i] = narrow<T>(drop<T, Residual>(
+                    widen<T>(x[first + i]), Residual ? widen<T>(residual[first + i]) : 0.0f, words[i / 4].w[i % 4],
+                    threshold, scale));
             }
         }
     }
 }
 
-// Pointers without 16-byte alignment: the same words, one element at a time.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) dropout_unaligned_kernel(
-    const T* x, const T* residual, long long total, uint32_t threshold, float scale, unsigned long long seed,
-    const unsigned long long* seed_device, unsigned long long offset, T* out
-) {
-    const long long first = (blockIdx.x * static_cast<long long>(kThreads) + threadIdx.x) * 4;
-    if (first >= total) {
-        return;
-    }
+template <typename T, int V, bool Aligned, bool Residual>
+void launch_dropout(const T* x, const T* residual, long long total, uint32_t threshold, float scale,
+                    unsigned long long seed, const unsigned long long* seed_device, unsigned long long offset, T* out,
+                    unsigned blocks, cudaStream_t stream) {
     if (seed_device != nullptr) {
-        seed = __ldg(seed_device);
-    }
-    const Words words = philox(static_cast<unsigned long long>(first) / 4, offset, seed);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (first + i < total) {
-            float v = words.w[i] >= threshold ? widen<T>(x[first + i]) * scale : 0.0f;
-            if (residual != nullptr) {
-                v += widen<T>(residual[first + i]);
-            }
-            out[first + i] = narrow<T>(v);
-        }
+        dropout_kernel<T, V, Aligned, Residual, true><<<blocks, kThreads, 0, stream>>>(
+            x, residual, total, threshold, scale, Keys{}, seed_device, offset, out);
+    } else {
+        dropout_kernel<T, V, Aligned, Residual, false><<<blocks, kThreads, 0, stream>>>(
+            x, residual, total, threshold, scale, round_keys(seed), nullptr, offset, out);
     }
 }
 
@@ -126,16 +143,19 @@ int run_dropout(const T* x, const T* residual, long long total, uint32_t thresho
                 unsigned long long seed, const unsigned long long* seed_device, unsigned long long offset, T* out,
                 cudaStream_t stream) {
     constexpr int V = 16 / sizeof(T);
-    const bool vec = aligned_to(x, 16) && aligned_to(residual, 16) && aligned_to(out, 16);
-    const long long per_block = static_cast<long long>(kThreads) * (vec ? V : 4);
+    const bool aligned = aligned_to(x, 16) && aligned_to(residual, 16) && aligned_to(out, 16);
+    const long long per_block = static_cast<long long>(kThreads) * V;
     const long long blocks = (total + per_block - 1) / per_block;
     LAT_REQUIRE(blocks <= 0x7fffffffLL, "dropout supports at most 2^31 blocks of elements.");
-    if (vec) {
-        dropout_kernel<T, V><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-            x, residual, total, threshold, scale, seed, seed_device, offset, out);
+    const unsigned grid = static_cast<unsigned>(blocks);
+    if (aligned && residual != nullptr) {
+        launch_dropout<T, V, true, true>(x, residual, total, threshold, scale, seed, seed_device, offset, out, grid, stream);
+    } else if (aligned) {
+        launch_dropout<T, V, true, false>(x, residual, total, threshold, scale, seed, seed_device, offset, out, grid, stream);
+    } else if (residual != nullptr) {
+        launch_dropout<T, V, false, true>(x, residual, total, threshold, scale, seed, seed_device, offset, out, grid, stream);
     } else {
-        dropout_unaligned_kernel<T><<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(
-            x, residual, total, threshold, scale, seed, seed_device, offset, out);
+        launch_dropout<T, V, false, false>(x, residual, total, threshold, scale, seed, seed_device, offset, out, grid, stream);
     }
     LAT_LAUNCH_CHECK();
     return LAT_OK;

@@ -27,6 +27,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "pairs.cuh"
 #include "vector_io.cuh"
 
 namespace lat {
@@ -74,33 +75,7 @@ struct Order {
     __device__ __forceinline__ int sequence(int j) const { return reverse ? sequences - 1 - j : j; }
 };
 
-// ---- arithmetic on pairs of channels: one instruction for two floats ----------------------
-
-struct alignas(8) Pair {
-    float x, y;
-};
-
-__device__ __forceinline__ Pair both(float v) { return {v, v}; }
-__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
-    Pair d;
-    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmul.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
-    Pair d;
-    asm("{\n.reg .b64 a, b, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nadd.rn.f32x2 d, a, b;\nmov.b64 {%0, %1}, d;\n}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
-    Pair d;
-    asm("{\n.reg .b64 a, b, c, d;\nmov.b64 a, {%2, %3};\nmov.b64 b, {%4, %5};\nmov.b64 c, {%6, %7};\n"
-        "fma.rn.f32x2 d, a, b, c;\nmov.b64 {%0, %1}, d;\n}"
-        : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-__device__ __forceinline__ Pair minus(Pair a, Pair b) { return fma(b, both(-1.0f), a); }   // a - b, rounded once
+// ---- gates -----------------------------------------------------------------------------
 
 __device__ __forceinline__ float exp2_fast(float v) {
     float r;

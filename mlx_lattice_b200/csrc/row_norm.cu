@@ -18,6 +18,7 @@
 #include <algorithm>
 
 #include "common.cuh"
+#include "pairs.cuh"
 #include "vector_io.cuh"
 
 namespace lat {
@@ -55,98 +56,150 @@ template <typename T> struct NormArgs {
 // thread waits for about 64 bytes of x at once (the memory needs some 50 KB in flight per SM).
 template <int K> constexpr int kRowsInFlight = K == 1 ? 4 : K <= 3 ? 2 : 1;
 
+// sum / count, correctly rounded but for the last place, and exactly the value of equal numbers:
+// the quotient by the reciprocal and one correction, a third of the instructions of a division.
+struct Count {
+    float n, inverse;
+
+    __device__ __forceinline__ explicit Count(int channels) : n(static_cast<float>(channels)), inverse(1.0f / n) {}
+    __device__ __forceinline__ float mean(float sum) const {
+        const float q = sum * inverse;
+        return fmaf(fmaf(-q, n, sum), inverse, q);
+    }
+};
+
+// The sums of all rows in flight over the lanes of a row, side by side.
+template <int U> __device__ __forceinline__ void group_sums(float (&v)[U], int lanes) {
+    for (int d = lanes >> 1; d > 0; d >>= 1) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            v[u] += __shfl_xor_sync(0xffffffffu, v[u], d);
+        }
+    }
+}
+
 // A lane owns the vectors lane, lane + L, ... of its row: K vectors of V elements.
 template <typename T, int V, int K, bool Rms>
 __global__ void __launch_bounds__(kThreads) norm_forward_kernel(NormArgs<T> p) {
-    constexpr int U = kRowsInFlight<K>;
+    constexpr int U = kRowsInFlight<K>, P = V == 1 ? 1 : V / 2;   // pairs of a vector; one may be half empty
     const int lane = threadIdx.x & 31;
     const int sub = lane & (p.lanes - 1);
     const int rows_per_warp = 32 / p.lanes;
-    const float count = static_cast<float>(p.channels);
+    const Count count(p.channels);
     const long long warp = blockIdx.x * static_cast<long long>(kWarps) + (threadIdx.x >> 5);
     const long long row0 = warp * rows_per_warp * U + lane / p.lanes;
-    Pack<T, V> x[U][K];
+    const int left = static_cast<int>(min(p.rows - row0, static_cast<long long>(U) * 32));   // rows from row0 on
+    const T* from = p.x + row0 * p.x_stride + sub * V;
+    const long long step = rows_per_warp * p.x_stride;
+    Pair x[U][K][P];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        const long long row = row0 + u * rows_per_warp;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            const int c = (sub + k * p.lanes) * V;
-            x[u][k] = row < p.rows && c < p.channels ? load_pack<T, V>(p.x + row * p.x_stride + c) : zero_pack<T, V>();
+            Pack<T, V> raw = zero_pack<T, V>();
+            if (u * rows_per_warp < left && (sub + k * p.lanes) * V < p.channels) {
+                raw = load_pack<T, V>(from + u * step + k * p.lanes * V);
+            }
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                x[u][k][i] = get_pair(raw, i);
+            }
         }
     }
     float mean[U], r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        float sum = 0.0f;
+        Pair sum = both(0.0f);
         if (!Rms) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    sum += x[u][k].get(i);
+                for (int i = 0; i < P; ++i) {
+                    sum = sum + x[u][k][i];
                 }
             }
         }
-        mean[u] = Rms ? 0.0f : group_sum(sum, p.lanes) / count;
+        mean[u] = sum.x + sum.y;
+    }
+    if (!Rms) {
+        group_sums(mean, p.lanes);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            mean[u] = count.mean(mean[u]);
+        }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        float squares = 0.0f;
+        Pair squares = both(0.0f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
             if ((sub + k * p.lanes) * V < p.channels) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float d = x[u][k].get(i) - mean[u];
-                    squares = fmaf(d, d, squares);
+                for (int i = 0; i < P; ++i) {
+                    if (!Rms) {
+                        x[u][k][i] = minus(x[u][k][i], V == 1 ? Pair{mean[u], 0.0f} : both(mean[u]));
+                    }
+                    squares = fma(x[u][k][i], x[u][k][i], squares);
                 }
             }
         }
-        r[u] = rsqrtf(group_sum(squares, p.lanes) / count + p.eps);
+        r[u] = squares.x + squares.y;
     }
-    if (sub == 0) {
+    group_sums(r, p.lanes);
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const long long row = row0 + u * rows_per_warp;
-            if (row < p.rows) {
-                p.rstd[row] = r[u];
-                if (!Rms) {
-                    p.mean[row] = mean[u];
-                }
+    for (int u = 0; u < U; ++u) {
+        r[u] = rsqrtf(fmaf(r[u], count.inverse, p.eps));
+        const long long row = row0 + u * rows_per_warp;
+        if (sub == 0 && u * rows_per_warp < left) {
+            p.rstd[row] = r[u];
+            if (!Rms) {
+                p.mean[row] = mean[u];
             }
         }
     }
+    T* to = p.out + row0 * p.channels + sub * V;
+    const long long down = static_cast<long long>(rows_per_warp) * p.channels;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = (sub + k * p.lanes) * V;
         if (c >= p.channels) {
             break;
         }
-        Pack<T, V> w, b;
+        Pair w[P], b[P];
         if (p.weight != nullptr) {
-            w = load_pack<T, V>(p.weight + c);
+            const Pack<T, V> raw = load_pack<T, V>(p.weight + c);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                w[i] = get_pair(raw, i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                w[i] = both(1.0f);
+            }
         }
         if (p.bias != nullptr) {
-            b = load_pack<T, V>(p.bias + c);
+            const Pack<T, V> raw = load_pack<T, V>(p.bias + c);
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                b[i] = get_pair(raw, i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < P; ++i) {
+                b[i] = both(0.0f);
+            }
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long row = row0 + u * rows_per_warp;
             Pack<T, V> y;
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                float v = (x[u][k].get(i) - mean[u]) * r[u];
-                if (p.weight != nullptr) {
-                    v *= w.get(i);
-                }
-                if (p.bias != nullptr) {
-                    v += b.get(i);
-                }
-                y.set(i, v);
+            for (int i = 0; i < P; ++i) {
+                const Pair xh = x[u][k][i] * both(r[u]);
+                set_pair(y, i, Rms ? xh * w[i] : fma(xh, w[i], b[i]));
             }
-            if (row < p.rows) {
-                store_pack<T, V>(p.out + row * p.channels + c, y);
+            if (u * rows_per_warp < left) {
+                store_pack<T, V>(to + u * down + k * p.lanes * V, y);
             }
         }
     }
@@ -154,78 +207,96 @@ __global__ void __launch_bounds__(kThreads) norm_forward_kernel(NormArgs<T> p) {
 
 template <typename T, int V, int K, bool Rms>
 __global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p, T* dw_out, T* db_out) {
-    constexpr int U = kRowsInFlight<K>;
+    constexpr int U = kRowsInFlight<K> > 2 ? 2 : kRowsInFlight<K>, P = V == 1 ? 1 : V / 2;
     extern __shared__ float sums[];  // [kWarps / 2][2][channels]
     const int lane = threadIdx.x & 31;
     const int sub = lane & (p.lanes - 1);
     const int rows_per_warp = 32 / p.lanes;
-    const float count = static_cast<float>(p.channels);
-    const long long step = static_cast<long long>(gridDim.x) * kWarps * rows_per_warp * U;
+    const Count count(p.channels);
     const int warp = threadIdx.x >> 5;
-    float dw[K][V], db[K][V];
-    Pack<T, V> w[K];
+    Pair dw[K][P], db[K][P], w[K][P];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
         const int c = (sub + k * p.lanes) * V;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            dw[k][i] = db[k][i] = 0.0f;
-            w[k].set(i, 1.0f);
+        Pack<T, V> raw;
+        const bool weighted = p.weight != nullptr && c < p.channels;
+        if (weighted) {
+            raw = load_pack<T, V>(p.weight + c);
         }
-        if (p.weight != nullptr && c < p.channels) {
-            w[k] = load_pack<T, V>(p.weight + c);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            dw[k][i] = db[k][i] = both(0.0f);
+            w[k][i] = weighted ? get_pair(raw, i) : both(1.0f);
         }
     }
+    const long long stride = static_cast<long long>(gridDim.x) * kWarps * rows_per_warp * U;
+    const long long x_step = rows_per_warp * p.x_stride, dy_step = rows_per_warp * p.dy_stride;
+    const long long down = static_cast<long long>(rows_per_warp) * p.channels;
     for (long long base = (blockIdx.x * static_cast<long long>(kWarps) + warp) * rows_per_warp * U; base < p.rows;
-         base += step) {
+         base += stride) {
         const long long row0 = base + lane / p.lanes;
-        Pack<T, V> x[U][K], dy[U][K];
-        float r[U], mean[U];
+        const int left = static_cast<int>(min(p.rows - row0, static_cast<long long>(U) * 32));
+        const T* x_from = p.x + row0 * p.x_stride + sub * V;
+        const T* dy_from = p.dy + row0 * p.dy_stride + sub * V;
+        T* to = p.out + row0 * p.channels + sub * V;
+        Pack<T, V> x_raw[U][K], dy_raw[U][K];
+        float r[U], mean[U], c1[U], c2[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long row = row0 + u * rows_per_warp;
-            const bool live = row < p.rows;
+            const bool live = u * rows_per_warp < left;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int c = (sub + k * p.lanes) * V;
-                const bool in = live && c < p.channels;
-                x[u][k] = in ? load_pack<T, V>(p.x + row * p.x_stride + c) : zero_pack<T, V>();
-                dy[u][k] = in ? load_pack<T, V>(p.dy + row * p.dy_stride + c) : zero_pack<T, V>();
+                const bool in = live && (sub + k * p.lanes) * V < p.channels;
+                x_raw[u][k] = in ? load_pack<T, V>(x_from + u * x_step + k * p.lanes * V) : zero_pack<T, V>();
+                dy_raw[u][k] = in ? load_pack<T, V>(dy_from + u * dy_step + k * p.lanes * V) : zero_pack<T, V>();
             }
-            r[u] = live ? p.rstd[row] : 0.0f;
-            mean[u] = !Rms && live ? p.mean[row] : 0.0f;
+            r[u] = live ? p.rstd[row0 + u * rows_per_warp] : 0.0f;
+            mean[u] = !Rms && live ? p.mean[row0 + u * rows_per_warp] : 0.0f;
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const long long row = row0 + u * rows_per_warp;
-            float c1 = 0.0f, c2 = 0.0f;
+            Pair s1 = both(0.0f), s2 = both(0.0f);
+            const Pair scale = both(r[u]), shift = both(mean[u]);
 #pragma unroll
             for (int k = 0; k < K; ++k) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
+                for (int i = 0; i < P; ++i) {
                     // zeros beyond the row's end: dy and with it every term is zero there
-                    const float d = dy[u][k].get(i);
-                    const float xh = (x[u][k].get(i) - mean[u]) * r[u];
-                    const float g = d * w[k].get(i);
-                    c1 += g;
-                    c2 = fmaf(g, xh, c2);
-                    dw[k][i] = fmaf(d, xh, dw[k][i]);
-                    db[k][i] += d;
+                    const Pair d = get_pair(dy_raw[u][k], i), x = get_pair(x_raw[u][k], i);
+                    const Pair xh = (Rms ? x : minus(x, shift)) * scale;
+                    const Pair g = d * w[k][i];
+                    if (!Rms) {
+                        s1 = s1 + g;
+                        db[k][i] = db[k][i] + d;
+                    }
+                    s2 = fma(g, xh, s2);
+                    dw[k][i] = fma(d, xh, dw[k][i]);
                 }
             }
-            c1 = Rms ? 0.0f : group_sum(c1, p.lanes) / count;
-            c2 = group_sum(c2, p.lanes) / count;
+            c1[u] = s1.x + s1.y;
+            c2[u] = s2.x + s2.y;
+        }
+        if (!Rms) {
+            group_sums(c1, p.lanes);
+        }
+        group_sums(c2, p.lanes);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            // r (g - c1 - xh c2) with xh = (x - m) r
+            const Pair scale = both(r[u]), shift = both(mean[u]);
+            const Pair minus_c1 = both(-count.mean(c1[u])), minus_c2 = both(-count.mean(c2[u]));
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int c = (sub + k * p.lanes) * V;
                 Pack<T, V> dx;
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float xh = (x[u][k].get(i) - mean[u]) * r[u];
-                    dx.set(i, r[u] * (dy[u][k].get(i) * w[k].get(i) - c1 - xh * c2));
+                for (int i = 0; i < P; ++i) {
+                    const Pair d = get_pair(dy_raw[u][k], i), x = get_pair(x_raw[u][k], i);
+                    const Pair xh = (Rms ? x : minus(x, shift)) * scale;
+                    const Pair g = Rms ? d * w[k][i] : fma(d, w[k][i], minus_c1);
+                    set_pair(dx, i, scale * fma(xh, minus_c2, g));
                 }
-                if (row < p.rows && c < p.channels) {
-                    store_pack<T, V>(p.out + row * p.channels + c, dx);
+                if (u * rows_per_warp < left && (sub + k * p.lanes) * V < p.channels) {
+                    store_pack<T, V>(to + u * down + k * p.lanes * V, dx);
                 }
             }
         }
@@ -239,9 +310,11 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p, 
 #pragma unroll
         for (int k = 0; k < K; ++k) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                dw[k][i] += __shfl_xor_sync(0xffffffffu, dw[k][i], d);
-                db[k][i] += __shfl_xor_sync(0xffffffffu, db[k][i], d);
+            for (int i = 0; i < P; ++i) {
+                dw[k][i].x += __shfl_xor_sync(0xffffffffu, dw[k][i].x, d);
+                dw[k][i].y += __shfl_xor_sync(0xffffffffu, dw[k][i].y, d);
+                db[k][i].x += __shfl_xor_sync(0xffffffffu, db[k][i].x, d);
+                db[k][i].y += __shfl_xor_sync(0xffffffffu, db[k][i].y, d);
             }
         }
     }
@@ -256,8 +329,10 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p, 
                 if (c < p.channels) {
 #pragma unroll
                     for (int i = 0; i < V; ++i) {
-                        mine[c + i] = phase == 0 ? dw[k][i] : dw[k][i] + mine[c + i];
-                        mine[p.channels + c + i] = phase == 0 ? db[k][i] : db[k][i] + mine[p.channels + c + i];
+                        const float w_sum = i % 2 == 0 ? dw[k][i / 2].x : dw[k][i / 2].y;
+                        const float b_sum = i % 2 == 0 ? db[k][i / 2].x : db[k][i / 2].y;
+                        mine[c + i] = phase == 0 ? w_sum : w_sum + mine[c + i];
+                        mine[p.channels + c + i] = phase == 0 ? b_sum : b_sum + mine[p.channels + c + i];
                     }
                 }
             }
@@ -470,7 +545,7 @@ template <typename T> int launch_reduce(const NormArgs<T>& p, int blocks, T* dw,
 template <typename T, int V, int K>
 int launch_backward(const NormArgs<T>& p, bool rms, T* dw, T* db, cudaStream_t stream) {
     const size_t smem = sizeof(float) * kWarps * p.channels;
-    const int grid = static_cast<int>(std::min<long long>(blocks_of(p.rows, p.lanes, kRowsInFlight<K>), kMaxBackwardBlocks));
+    const int grid = static_cast<int>(std::min<long long>(blocks_of(p.rows, p.lanes, kRowsInFlight<K> > 2 ? 2 : kRowsInFlight<K>), kMaxBackwardBlocks));
     if (rms) {
         norm_backward_kernel<T, V, K, true><<<grid, kThreads, smem, stream>>>(p, dw, db);
     } else {
@@ -616,6 +691,7 @@ int lat_row_norm_backward(
     LAT_REQUIRE(dtype == LAT_F32 || dtype == LAT_F16, "normalisation supports float32 and float16 tensors.");
     LAT_REQUIRE(rows >= 0 && channels > 0 && feat_row_stride >= 0 && grad_row_stride >= 0,
                 "feats must have shape (N, C).");
+    LAT_REQUIRE(!rms || grad_bias == nullptr, "rms_norm has no bias.");
     const bool sums = grad_weight != nullptr || grad_bias != nullptr;
     cudaStream_t stream = as_stream(stream_ptr);
     const size_t element = dtype == LAT_F32 ? 4 : 2;

@@ -27,6 +27,8 @@ def test_row_norm_entry_points_refuse_bad_arguments():
     _refused(lib.lat_row_norm_forward(F32, 0, buf, 4, 8, 8, None, None, 1e-5, buf, None, buf, None), 'statistics')
     _refused(lib.lat_row_norm_backward(F32, 0, buf, 8, buf, 4, 8, 8, None, None, buf, buf, None, None, None, 0, None),
              'statistics of the forward pass')
+    _refused(lib.lat_row_norm_backward(F32, 1, buf, 8, buf, 4, 8, 8, None, None, buf, buf, None, buf, None, 0, None),
+             'no bias')
     need = lib.lat_row_norm_backward_workspace_bytes(4, 8)
     assert lib.lat_row_norm_backward(F32, 0, buf, 8, buf, 4, 8, 8, None, buf, buf, buf, buf, None, buf, need - 1,
                                      None) == _native.LAT_WORKSPACE_TOO_SMALL
