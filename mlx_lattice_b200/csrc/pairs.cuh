@@ -39,7 +39,7 @@ template <typename T, int V> __device__ __forceinline__ Pair get_pair(const Pack
     if constexpr (V == 1) {
         return {p.get(0), 0.0f};
     } else if constexpr (sizeof(T) == 2) {
-        const float2 f = __half22float2(__halves2half2(p.v[2 * i], p.v[2 * i + 1]));
+        const float2 f = __half22float2(reinterpret_cast<const __half2*>(p.v)[i]);
         return {f.x, f.y};
     } else {
         return {p.v[2 * i], p.v[2 * i + 1]};
@@ -50,9 +50,7 @@ template <typename T, int V> __device__ __forceinline__ void set_pair(Pack<T, V>
     if constexpr (V == 1) {
         p.set(0, value.x);
     } else if constexpr (sizeof(T) == 2) {
-        const __half2 h = __floats2half2_rn(value.x, value.y);
-        p.v[2 * i] = __low2half(h);
-        p.v[2 * i + 1] = __high2half(h);
+        reinterpret_cast<__half2*>(p.v)[i] = __floats2half2_rn(value.x, value.y);
     } else {
         p.v[2 * i] = value.x;
         p.v[2 * i + 1] = value.y;

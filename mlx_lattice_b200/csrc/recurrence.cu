@@ -238,7 +238,7 @@ template <int N> struct Row {
 #pragma unroll
         for (int i = 0; i < kPairs; ++i) {
             if constexpr (sizeof(T) == 2) {
-                const float2 f = __half22float2(__halves2half2(raw.v[2 * i], raw.v[2 * i + 1]));
+                const float2 f = __half22float2(reinterpret_cast<const __half2*>(raw.v)[i]);
                 out.v[i] = {f.x, f.y};
             } else {
                 out.v[i] = {raw.v[2 * i], raw.v[2 * i + 1]};
@@ -285,9 +285,7 @@ template <typename T, int N, int Granule> struct Channels {
 #pragma unroll
         for (int i = 0; i < N / 2; ++i) {
             if constexpr (sizeof(T) == 2) {
-                const __half2 h = __floats2half2_rn(value.v[i].x, value.v[i].y);
-                raw.v[2 * i] = __low2half(h);
-                raw.v[2 * i + 1] = __high2half(h);
+                reinterpret_cast<__half2*>(raw.v)[i] = __floats2half2_rn(value.v[i].x, value.v[i].y);
             } else {
                 raw.v[2 * i] = value.v[i].x;
                 raw.v[2 * i + 1] = value.v[i].y;
