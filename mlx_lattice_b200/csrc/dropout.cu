@@ -52,8 +52,8 @@ __device__ __forceinline__ void multiply(uint32_t a, uint32_t b, uint32_t& low, 
     asm("{\n.reg .b64 p;\nmul.wide.u32 p, %2, %3;\nmov.b64 {%0, %1}, p;\n}" : "=r"(low), "=r"(high) : "r"(a), "r"(b));
 }
 
-__device__ __forceinline__ Words philox(unsigned long long index, unsigned long long offset, const Keys& keys) {
-    uint32_t c0 = static_cast<uint32_t>(index), c1 = static_cast<uint32_t>(index >> 32);
+__device__ __forceinline__ Words philox(uint32_t low, uint32_t high, unsigned long long offset, const Keys& keys) {
+    uint32_t c0 = low, c1 = high;
     uint32_t c2 = static_cast<uint32_t>(offset), c3 = static_cast<uint32_t>(offset >> 32);
 #pragma unroll
     for (int round = 0; round < kRounds; ++round) {
@@ -99,10 +99,14 @@ __global__ void __launch_bounds__(kThreads) dropout_kernel(
     if (DeviceSeed) {
         keys = round_keys(__ldg(seed));
     }
+    // A block's counters share their upper word, as a block has a power of two of them: two of the
+    // 20 products are then the same for the whole block.
+    const unsigned long long counter = blockIdx.x * static_cast<unsigned long long>(kThreads * V / 4);
+    const uint32_t low = static_cast<uint32_t>(counter) + threadIdx.x * (V / 4);
     Words words[V / 4];
 #pragma unroll
     for (int q = 0; q < V / 4; ++q) {
-        words[q] = philox(static_cast<unsigned long long>(first) / 4 + q, offset, keys);
+        words[q] = philox(low + q, static_cast<uint32_t>(counter >> 32), offset, keys);
     }
     if (whole) {
 #pragma unroll
