@@ -62,6 +62,7 @@ Matrix matrix(const Tensor& t, const char* name) {
     require_cuda(t, name);
     REQUIRE(t.dim() == 2, name, " must have shape (N, C).");
     Tensor dense = t.stride(1) == 1 ? t : t.contiguous();
+    REQUIRE(t.size(1) <= 0x7fffffff, name, " has too many channels.");
     const int64_t stride = dense.size(0) > 1 ? dense.stride(0) : dense.size(1);
     return {dense, dense.size(0), dense.size(1), stride};
 }
@@ -294,11 +295,12 @@ Tensor offsets_argument(const Tensor& t, const Matrix& like) {
     REQUIRE(t.scalar_type() == at::kInt, "offsets must be int32.");
     REQUIRE(t.dim() == 1 && t.numel() >= 1 && t.device() == like.t.device(),
                       "offsets must hold one int32 entry per sequence and one more, on the feature device.");
+    REQUIRE(t.numel() <= 0x7fffffff, "offsets has too many entries.");
     return t.contiguous();
 }
 
 void check_rows(const Matrix& feats) {
-    REQUIRE(feats.rows <= 0x7fffffff && feats.channels <= 0x7fffffff, "feats has too many rows.");
+    REQUIRE(feats.rows <= 0x7fffffff, "feats has too many rows.");
 }
 
 std::tuple<Tensor, Tensor, Tensor> recurrence_forward(
@@ -381,6 +383,22 @@ struct Recurrence : torch::autograd::Function<Recurrence> {
     }
 };
 
+// Whether the ranges of memory that two tensors span have a byte in common.
+bool overlap(const Tensor& a, const Tensor& b) {
+    if (a.numel() == 0 || b.numel() == 0) {
+        return false;
+    }
+    const auto begin = [](const Tensor& t) { return reinterpret_cast<uintptr_t>(t.const_data_ptr()); };
+    const auto end = [&](const Tensor& t) {
+        int64_t last = 0;
+        for (int64_t d = 0; d < t.dim(); ++d) {
+            last += (t.size(d) - 1) * t.stride(d);
+        }
+        return begin(t) + (last + 1) * t.element_size();
+    };
+    return begin(a) < end(b) && begin(b) < end(a);
+}
+
 std::tuple<Tensor, Tensor> recurrence_step(
     const Tensor& feats_in, const Tensor& gate_in, const OptionalTensor& state_in, const OptionalTensor& out_state_in
 ) {
@@ -392,10 +410,14 @@ std::tuple<Tensor, Tensor> recurrence_step(
     Tensor next = out_state_in.value_or(Tensor());
     if (next.defined()) {
         REQUIRE(state_argument(next, "out_state", feats.rows, feats).is_same(next), "out_state must be contiguous.");
+        // a thread reads and writes one place of the state; every other overlap is a race
+        REQUIRE(next.const_data_ptr() == state.const_data_ptr() || !overlap(next, state),
+                "out_state must be state or lie apart from it.");
+        REQUIRE(!overlap(next, feats.t) && !overlap(next, gate.t), "out_state must lie apart from the features and the gate.");
+        next.unsafeGetTensorImpl()->bump_version();   // written in place
     } else {
         next = new_floats(feats, {feats.rows, feats.channels});
     }
-    REQUIRE(feats.channels <= 0x7fffffff, "feats has too many channels.");
     const Tensor out = new_like(feats, {feats.rows, feats.channels});
     const c10::cuda::CUDAGuard guard(feats.t.device());
     check(lat_recurrence_step(

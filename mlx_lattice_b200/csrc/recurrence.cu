@@ -884,6 +884,8 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(
 
 constexpr int kMaxRows = 0x7fffffff - kTileRows;   // row numbers of the last tile stay in an int
 
+constexpr int kMaxChannels = 65535 * kScanChannels;   // of the scan kernel's grid
+
 inline int tiles_of(long long rows) { return static_cast<int>((rows + kTileRows - 1) / kTileRows); }
 
 // Threads across a slab for so many threads' worth of channels: `most`, a 128-byte line, or half
@@ -961,7 +963,6 @@ int launch_scan(ScanArgs<T> p, void* workspace, size_t bytes, cudaStream_t strea
             return code;
         }
         const dim3 scan_grid((groups + kWindow - 1) / kWindow, (p.channels + kScanChannels - 1) / kScanChannels);
-        LAT_REQUIRE(scan_grid.y <= 65535, "the recurrence supports at most two million channels.");
         recurrence_scan_kernel<<<scan_grid, 32 * kScanWarps, 0, stream>>>(p.groups, groups, p.channels, p.windows,
                                                                           p.states, p.arrived);
         LAT_LAUNCH_CHECK();
@@ -1095,6 +1096,7 @@ int lat_recurrence_forward(
     LAT_REQUIRE(dtype == LAT_F32 || dtype == LAT_F16, "the recurrence supports float32 and float16 tensors.");
     LAT_REQUIRE(rows >= 0 && rows <= kMaxRows && channels > 0 && feat_row_stride >= 0 && gate_row_stride >= 0,
                 "feats and gate must have shape (N, C).");
+    LAT_REQUIRE(channels <= kMaxChannels, "the recurrence supports at most 2097120 channels.");
     LAT_REQUIRE(sequences >= 0 && (sequences == 0 || offsets != nullptr),
                 "offsets must hold one int32 entry per sequence and one more.");
     cudaStream_t stream = as_stream(stream_ptr);
@@ -1122,6 +1124,7 @@ int lat_recurrence_backward(
     LAT_REQUIRE(dtype == LAT_F32 || dtype == LAT_F16, "the recurrence supports float32 and float16 tensors.");
     LAT_REQUIRE(rows >= 0 && rows <= kMaxRows && channels > 0 && feat_row_stride >= 0 && gate_row_stride >= 0 &&
                     grad_row_stride >= 0, "feats and gate must have shape (N, C).");
+    LAT_REQUIRE(channels <= kMaxChannels, "the recurrence supports at most 2097120 channels.");
     LAT_REQUIRE(sequences >= 0 && (sequences == 0 || offsets != nullptr),
                 "offsets must hold one int32 entry per sequence and one more.");
     cudaStream_t stream = as_stream(stream_ptr);

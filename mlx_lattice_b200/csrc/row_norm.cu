@@ -586,9 +586,11 @@ __global__ void __launch_bounds__(kThreads, kForwardBlocks<16 / sizeof(T), K>) n
 }
 
 // Element by element, for rows that do not come in 16-byte vectors.
-template <typename T, int V, int K, bool Rms>
+template <int K> constexpr int kPlainRows = K <= 3 ? 2 : 1;   // of a thread in flight
+
+template <typename T, int K, bool Rms>
 __global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p, T* dw_out, T* db_out) {
-    constexpr int U = kRowsInFlight<K> > 2 ? 2 : kRowsInFlight<K>, P = V == 1 ? 1 : V / 2;
+    constexpr int V = 1, U = kPlainRows<K>, P = 1;
     extern __shared__ float sums[];  // [kWarps / 2][2][channels]
     const int lane = threadIdx.x & 31;
     const int sub = lane & (p.lanes - 1);
@@ -869,6 +871,7 @@ int launch_forward(const NormArgs<T>& p, bool rms, cudaStream_t stream) {
 }
 
 constexpr int kMaxBackwardBlocks = 148 * 3;
+constexpr int kMaxChannels = 65535 * kThreads;   // of the sums' grid
 
 template <typename T> int launch_reduce(const NormArgs<T>& p, int blocks, T* dw, T* db, cudaStream_t stream) {
     norm_reduce_kernel<T><<<(2 * p.channels + 31) / 32, 32 * kReduceParts, 0, stream>>>(
@@ -882,11 +885,11 @@ int launch_backward(const NormArgs<T>& p, bool rms, T* dw, T* db, cudaStream_t s
     const size_t sums = sizeof(float) * kWarps * p.channels;
     int grid;
     if constexpr (V == 1) {
-        grid = static_cast<int>(std::min<long long>(blocks_of(p.rows, p.lanes, kRowsInFlight<K> > 2 ? 2 : kRowsInFlight<K>), 148 * 2));
+        grid = static_cast<int>(std::min<long long>(blocks_of(p.rows, p.lanes, kPlainRows<K>), 148 * 2));
         if (rms) {
-            norm_backward_kernel<T, V, K, true><<<grid, kThreads, sums, stream>>>(p, dw, db);
+            norm_backward_kernel<T, K, true><<<grid, kThreads, sums, stream>>>(p, dw, db);
         } else {
-            norm_backward_kernel<T, V, K, false><<<grid, kThreads, sums, stream>>>(p, dw, db);
+            norm_backward_kernel<T, K, false><<<grid, kThreads, sums, stream>>>(p, dw, db);
         }
     } else {
         grid = static_cast<int>(std::min<long long>(blocks_of(p.rows, p.lanes, kRingRows<K>), 148 * kRingBlocks<V, K>));
@@ -971,7 +974,6 @@ int run_backward(const NormArgs<T>& p, bool rms, T* dw, T* db, cudaStream_t stre
     const long long per_block = (p.rows + partial_rows(p.rows) - 1) / partial_rows(p.rows);
     const int blocks = static_cast<int>((p.rows + per_block - 1) / per_block);
     const dim3 sums_grid(blocks, (p.channels + kThreads - 1) / kThreads);
-    LAT_REQUIRE(sums_grid.y <= 65535, "normalisation supports at most 16 million channels.");
     if (rms) {
         norm_sums_wide_kernel<T, true><<<sums_grid, kThreads, 0, stream>>>(p, per_block);
     } else {
@@ -1005,6 +1007,7 @@ int lat_row_norm_forward(
     LAT_REQUIRE(dtype == LAT_F32 || dtype == LAT_F16, "normalisation supports float32 and float16 tensors.");
     LAT_REQUIRE(eps > 0.0f, "eps must be positive.");
     LAT_REQUIRE(rows >= 0 && channels > 0 && feat_row_stride >= 0, "feats must have shape (N, C).");
+    LAT_REQUIRE(channels <= kMaxChannels, "normalisation supports at most 16776960 channels.");
     LAT_REQUIRE(!rms || bias == nullptr, "rms_norm has no bias.");
     if (rows == 0) {
         return LAT_OK;
@@ -1035,6 +1038,7 @@ int lat_row_norm_backward(
     LAT_REQUIRE(dtype == LAT_F32 || dtype == LAT_F16, "normalisation supports float32 and float16 tensors.");
     LAT_REQUIRE(rows >= 0 && channels > 0 && feat_row_stride >= 0 && grad_row_stride >= 0,
                 "feats must have shape (N, C).");
+    LAT_REQUIRE(channels <= kMaxChannels, "normalisation supports at most 16776960 channels.");
     LAT_REQUIRE(!rms || grad_bias == nullptr, "rms_norm has no bias.");
     const bool sums = grad_weight != nullptr || grad_bias != nullptr;
     cudaStream_t stream = as_stream(stream_ptr);

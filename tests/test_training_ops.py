@@ -75,6 +75,20 @@ def test_recurrence_entry_points_refuse_bad_arguments():
     assert [lib.lat_recurrence_carry_rows(n) for n in (-1, 0, 1, 8, 9)] == [0, 0, 1, 1, 2]
 
 
+def test_rows_too_wide_for_a_launch_are_refused_before_it():
+    lib = _native.load()
+    buf = ctypes.c_void_p(4096)
+    wide = 65535 * 256 + 1
+    _refused(lib.lat_row_norm_forward(F32, 0, buf, 4, wide, wide, None, None, 1e-5, buf, buf, buf, None), 'channels')
+    _refused(lib.lat_row_norm_backward(F16, 1, buf, wide, buf, 4, wide, wide, None, None, buf, buf, None, None, None, 0,
+                                       None), 'channels')
+    wide = 65535 * 32 + 1
+    _refused(lib.lat_recurrence_forward(F32, buf, wide, buf, wide, 4, wide, buf, 1, None, 0, buf, None, None, buf,
+                                        1 << 62, None, None), 'channels')
+    _refused(lib.lat_recurrence_backward(F32, buf, wide, None, buf, wide, buf, wide, 4, wide, buf, 1, None, 0, buf, buf,
+                                         buf, None, buf, 1 << 62, None, None), 'channels')
+
+
 def test_host_tensors_are_refused():
     x = torch.zeros((4, 8))
     for call in (lambda: _ext.row_norm_forward(x, None, None, 1e-5, False),

@@ -586,6 +586,30 @@ def test_recurrence_step_continues_a_sequence(cuda, dtype, rows, channels):
     assert _ext.recurrence_step(x[:0], z[:0], state[:0])[0].shape == (0, channels)
 
 
+def test_recurrence_step_into_a_given_state(cuda):
+    """The next state may take the place of the state, or lie apart from all inputs; a graph that
+    keeps the overwritten state for its gradient notices."""
+    from mlx_lattice_b200 import ops
+
+    feats = torch.ones((16, 8), device=cuda)
+    x, pool = _sparse(feats), torch.zeros((64, 8), device=cuda)
+    _, apart = ops.gated_recurrence_step(x, feats, pool[:16], out_state=pool[16:32])
+    _, placed = ops.gated_recurrence_step(x, feats, pool[:16], out_state=pool[:16])
+    assert torch.equal(apart, placed) and not pool[32:].any()
+    with pytest.raises(ValueError, match='apart from it'):
+        ops.gated_recurrence_step(x, feats, pool[:16], out_state=pool[8:24])
+    for x_rows, gate in ((pool[32:48], feats), (feats, pool[40:56])):
+        with pytest.raises(ValueError, match='apart from the features'):
+            ops.gated_recurrence_step(_sparse(x_rows), gate, pool[:16], out_state=pool[32:48])
+    state = torch.zeros((1, 8), device=cuda)
+    leaf = feats.clone().requires_grad_(True)
+    y = ops.gated_recurrence(_sparse(leaf), feats, initial_state=state,
+                             offsets=torch.tensor([0, 16], dtype=torch.int32, device=cuda)).feats
+    ops.gated_recurrence_step(_sparse(feats[:1]), feats[:1], state, out_state=state)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        y.sum().backward()
+
+
 def test_prefill_then_steps(cuda):
     """A cloud's rows in one call, or a part of them and then row by row from the state."""
     from mlx_lattice_b200 import ops
