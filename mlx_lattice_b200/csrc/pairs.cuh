@@ -36,9 +36,7 @@ __device__ __forceinline__ Pair minus(Pair a, Pair b) { return fma(b, both(-1.0f
 
 // elements 2 i and 2 i + 1 of a pack
 template <typename T, int V> __device__ __forceinline__ Pair get_pair(const Pack<T, V>& p, int i) {
-    if constexpr (V == 1) {
-        return {p.get(0), 0.0f};
-    } else if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2) {
         const float2 f = __half22float2(reinterpret_cast<const __half2*>(p.v)[i]);
         return {f.x, f.y};
     } else {
@@ -47,9 +45,7 @@ template <typename T, int V> __device__ __forceinline__ Pair get_pair(const Pack
 }
 
 template <typename T, int V> __device__ __forceinline__ void set_pair(Pack<T, V>& p, int i, Pair value) {
-    if constexpr (V == 1) {
-        p.set(0, value.x);
-    } else if constexpr (sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2) {
         reinterpret_cast<__half2*>(p.v)[i] = __floats2half2_rn(value.x, value.y);
     } else {
         p.v[2 * i] = value.x;

@@ -6,10 +6,17 @@
 //   g = dy w:  dx = r (g - mean(g) [layer only] - xh mean(g xh))
 //   dw = sum over rows of dy xh, db = sum over rows of dy
 //
-// Both passes are bound by the memory: the forward pass reads x and writes y, the backward
-// pass reads x and dy and writes dx. A group of L lanes (a power of two) holds a row in
-// registers, so every element is read once and the variance is taken about the mean in a
-// second pass over registers. All sums are float32; results are rounded once.
+// The forward pass reads x and writes y, the backward pass reads x and dy and writes dx. A group
+// of L lanes (a power of two) holds a row in registers or in its own part of shared memory, so
+// every element is read once and the variance is taken about the mean in a second pass over what
+// is held. All sums are float32; results are rounded once.
+//
+// Both are bound by the memory, or nearly so (a copy moves 6.55 TB/s):
+//   960,000 x 64 float16, layer   forward 41 us, 5.9 TB/s   backward 64 us + sums 3 us, 5.7 TB/s
+//   240,001 x 192 float16, RMS    forward 28 us, 6.5 TB/s   backward 49 us + sums 3 us, 5.6 TB/s
+//   30,011 x 1000 float32, layer  forward 40 us, 6.0 TB/s   backward 61 us + sums 3 us, 5.9 TB/s
+// What the backward pass of narrow rows still loses is instructions: two shuffle trees a row and
+// the sums down the rows.
 //
 // The gradients of weight and bias are sums down the rows. Every lane keeps the sums of the
 // channels it owns over all rows it visits, a block adds its lanes' sums up in a fixed order
@@ -52,9 +59,64 @@ template <typename T> struct NormArgs {
     float* partial;   // [gridDim.x][2][channels]
 };
 
-// Rows that a group of lanes has in flight: with K vectors a lane, enough of them that a
-// thread waits for about 64 bytes of x at once (the memory needs some 50 KB in flight per SM).
-template <int K> constexpr int kRowsInFlight = K == 1 ? 4 : K <= 3 ? 2 : 1;
+// Rows that a group of lanes has in flight where a lane takes so many bytes of each: enough of
+// them that a thread waits for about 64 bytes of x at once (the memory needs some 50 KB in flight
+// per SM).
+template <int Bytes> constexpr int kRowsInFlight = Bytes <= 8 ? 8 : Bytes <= 16 ? 4 : Bytes <= 48 ? 2 : 1;
+
+// How a lane's part of a row moves: vectors of V elements, every L-th of the row, one a step; for
+// V = 1 two elements a step, L apart, which are computed as one pair.
+template <typename T, int V> struct Columns {
+    static constexpr int kWidth = V == 1 ? 2 : V;   // elements of a step
+    using Raw = Pack<T, kWidth>;
+    int first, lanes, channels;
+
+    __device__ __forceinline__ Columns(int sub, int lanes, int channels) : first(sub * V), lanes(lanes), channels(channels) {}
+    // element i of step k
+    __device__ __forceinline__ int at(int k, int i) const { return first + k * lanes * kWidth + (V == 1 ? i * lanes : i); }
+    __device__ __forceinline__ bool has(int k, int i = 0) const { return at(k, i) < channels; }
+    __device__ __forceinline__ Raw load(const T* row, int k) const {
+        if constexpr (V == 1) {
+            Raw raw = zero_pack<T, kWidth>();
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (has(k, i)) {
+                    raw.v[i] = row[at(k, i)];
+                }
+            }
+            return raw;
+        } else {
+            return has(k) ? load_pack<T, V>(row + at(k, 0)) : zero_pack<T, V>();
+        }
+    }
+    __device__ __forceinline__ void store(T* row, int k, const Raw& raw) const {
+        if constexpr (V == 1) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                if (has(k, i)) {
+                    row[at(k, i)] = raw.v[i];
+                }
+            }
+        } else if (has(k)) {
+            store_pack<T, V>(row + at(k, 0), raw);
+        }
+    }
+    // a step of a vector of the row's length, or `value` without one
+    __device__ __forceinline__ void vector(const T* from, int k, float value, Pair (&to)[kWidth / 2]) const {
+        Raw raw = zero_pack<T, kWidth>();
+        if (from != nullptr) {
+            raw = load(from, k);
+        }
+#pragma unroll
+        for (int i = 0; i < kWidth / 2; ++i) {
+            to[i] = from != nullptr ? get_pair(raw, i) : both(value);
+        }
+    }
+    // a step with zeros behind the row's end
+    __device__ __forceinline__ Pair within(int k, Pair value) const {
+        return {has(k) ? value.x : 0.0f, (V == 1 ? has(k, 1) : has(k)) ? value.y : 0.0f};
+    }
+};
 
 // sum / count, correctly rounded but for the last place, and exactly the value of equal numbers:
 // the quotient by the reciprocal and one correction, a third of the instructions of a division.
@@ -78,28 +140,28 @@ template <int U> __device__ __forceinline__ void group_sums(float (&v)[U], int l
     }
 }
 
-// A lane owns the vectors lane, lane + L, ... of its row: K vectors of V elements.
+// All rows of a thread are loaded before the first is used. For float32, and element by element
+// (V = 1) for rows of no vectors that lie apart or off a 16-byte boundary.
 template <typename T, int V, int K, bool Rms>
 __global__ void __launch_bounds__(kThreads) norm_forward_kernel(NormArgs<T> p) {
-    constexpr int U = kRowsInFlight<K>, P = V == 1 ? 1 : V / 2;   // pairs of a vector; one may be half empty
+    using Lane = Columns<T, V>;
+    constexpr int U = kRowsInFlight<Lane::kWidth * K * sizeof(T)>, P = Lane::kWidth / 2;
     const int lane = threadIdx.x & 31;
     const int sub = lane & (p.lanes - 1);
     const int rows_per_warp = 32 / p.lanes;
+    const Lane columns(sub, p.lanes, p.channels);
     const Count count(p.channels);
     const long long warp = blockIdx.x * static_cast<long long>(kWarps) + (threadIdx.x >> 5);
     const long long row0 = warp * rows_per_warp * U + lane / p.lanes;
     const int left = static_cast<int>(min(p.rows - row0, static_cast<long long>(U) * 32));   // rows from row0 on
-    const T* from = p.x + row0 * p.x_stride + sub * V;
+    const T* from = p.x + row0 * p.x_stride;
     const long long step = rows_per_warp * p.x_stride;
     Pair x[U][K][P];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            Pack<T, V> raw = zero_pack<T, V>();
-            if (u * rows_per_warp < left && (sub + k * p.lanes) * V < p.channels) {
-                raw = load_pack<T, V>(from + u * step + k * p.lanes * V);
-            }
+            const auto raw = u * rows_per_warp < left ? columns.load(from + u * step, k) : zero_pack<T, Lane::kWidth>();
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 x[u][k][i] = get_pair(raw, i);
@@ -133,14 +195,12 @@ __global__ void __launch_bounds__(kThreads) norm_forward_kernel(NormArgs<T> p) {
         Pair squares = both(0.0f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            if ((sub + k * p.lanes) * V < p.channels) {
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    if (!Rms) {
-                        x[u][k][i] = minus(x[u][k][i], V == 1 ? Pair{mean[u], 0.0f} : both(mean[u]));
-                    }
-                    squares = fma(x[u][k][i], x[u][k][i], squares);
+            for (int i = 0; i < P; ++i) {
+                if (!Rms) {
+                    x[u][k][i] = columns.within(k, minus(x[u][k][i], both(mean[u])));
                 }
+                squares = fma(x[u][k][i], x[u][k][i], squares);
             }
         }
         r[u] = squares.x + squares.y;
@@ -157,49 +217,26 @@ __global__ void __launch_bounds__(kThreads) norm_forward_kernel(NormArgs<T> p) {
             }
         }
     }
-    T* to = p.out + row0 * p.channels + sub * V;
+    T* to = p.out + row0 * p.channels;
     const long long down = static_cast<long long>(rows_per_warp) * p.channels;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int c = (sub + k * p.lanes) * V;
-        if (c >= p.channels) {
+        if (!columns.has(k)) {
             break;
         }
         Pair w[P], b[P];
-        if (p.weight != nullptr) {
-            const Pack<T, V> raw = load_pack<T, V>(p.weight + c);
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                w[i] = get_pair(raw, i);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                w[i] = both(1.0f);
-            }
-        }
-        if (p.bias != nullptr) {
-            const Pack<T, V> raw = load_pack<T, V>(p.bias + c);
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                b[i] = get_pair(raw, i);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < P; ++i) {
-                b[i] = both(0.0f);
-            }
-        }
+        columns.vector(p.weight, k, 1.0f, w);
+        columns.vector(p.bias, k, 0.0f, b);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            Pack<T, V> y;
+            typename Lane::Raw y;
 #pragma unroll
             for (int i = 0; i < P; ++i) {
                 const Pair xh = x[u][k][i] * both(r[u]);
                 set_pair(y, i, Rms ? xh * w[i] : fma(xh, w[i], b[i]));
             }
             if (u * rows_per_warp < left) {
-                store_pack<T, V>(to + u * down + k * p.lanes * V, y);
+                columns.store(to + u * down, k, y);
             }
         }
     }
@@ -212,7 +249,9 @@ template <typename T, int V, int K, int P>
 __device__ __forceinline__ void finish_sums(
     const NormArgs<T>& p, Pair (&dw)[K][P], Pair (&db)[K][P], float* sums, T* dw_out, T* db_out
 ) {
-    const int lane = threadIdx.x & 31, sub = lane & (p.lanes - 1), warp = threadIdx.x >> 5;
+    using Lane = Columns<T, V>;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const Lane columns(lane & (p.lanes - 1), p.lanes, p.channels);
     if (dw_out == nullptr && db_out == nullptr) {
         return;
     }
@@ -235,14 +274,14 @@ __device__ __forceinline__ void finish_sums(
         if ((warp >= kHalf) == (phase == 0) && lane < p.lanes) {
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const int c = (sub + k * p.lanes) * V;
-                if (c < p.channels) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) {
+                for (int i = 0; i < Lane::kWidth; ++i) {
+                    const int c = columns.at(k, i);
+                    if (c < p.channels) {
                         const float w_sum = i % 2 == 0 ? dw[k][i / 2].x : dw[k][i / 2].y;
                         const float b_sum = i % 2 == 0 ? db[k][i / 2].x : db[k][i / 2].y;
-                        mine[c + i] = phase == 0 ? w_sum : w_sum + mine[c + i];
-                        mine[p.channels + c + i] = phase == 0 ? b_sum : b_sum + mine[p.channels + c + i];
+                        mine[c] = phase == 0 ? w_sum : w_sum + mine[c];
+                        mine[p.channels + c] = phase == 0 ? b_sum : b_sum + mine[p.channels + c];
                     }
                 }
             }
@@ -585,31 +624,28 @@ __global__ void __launch_bounds__(kThreads, kForwardBlocks<16 / sizeof(T), K>) n
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Element by element, for rows that do not come in 16-byte vectors.
-template <int K> constexpr int kPlainRows = K <= 3 ? 2 : 1;   // of a thread in flight
+// For rows of no vectors that lie apart or off a 16-byte boundary, element by element.
+template <int Bytes> constexpr int kBackwardRows = Bytes <= 8 ? 4 : Bytes <= 16 ? 2 : 1;
 
 template <typename T, int K, bool Rms>
-__global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p, T* dw_out, T* db_out) {
-    constexpr int V = 1, U = kPlainRows<K>, P = 1;
+__global__ void __launch_bounds__(kThreads, K <= 6 ? 2 : 1) norm_backward_kernel(NormArgs<T> p, T* dw_out, T* db_out) {
+    constexpr int V = 1;
+    using Lane = Columns<T, V>;
+    constexpr int U = kBackwardRows<Lane::kWidth * K * sizeof(T)>, P = Lane::kWidth / 2;
     extern __shared__ float sums[];  // [kWarps / 2][2][channels]
     const int lane = threadIdx.x & 31;
     const int sub = lane & (p.lanes - 1);
     const int rows_per_warp = 32 / p.lanes;
+    const Lane columns(sub, p.lanes, p.channels);
     const Count count(p.channels);
     const int warp = threadIdx.x >> 5;
     Pair dw[K][P], db[K][P], w[K][P];
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-        const int c = (sub + k * p.lanes) * V;
-        Pack<T, V> raw;
-        const bool weighted = p.weight != nullptr && c < p.channels;
-        if (weighted) {
-            raw = load_pack<T, V>(p.weight + c);
-        }
+        columns.vector(p.weight, k, 1.0f, w[k]);
 #pragma unroll
         for (int i = 0; i < P; ++i) {
             dw[k][i] = db[k][i] = both(0.0f);
-            w[k][i] = weighted ? get_pair(raw, i) : both(1.0f);
         }
     }
     const long long stride = static_cast<long long>(gridDim.x) * kWarps * rows_per_warp * U;
@@ -619,19 +655,18 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p, 
          base += stride) {
         const long long row0 = base + lane / p.lanes;
         const int left = static_cast<int>(min(p.rows - row0, static_cast<long long>(U) * 32));
-        const T* x_from = p.x + row0 * p.x_stride + sub * V;
-        const T* dy_from = p.dy + row0 * p.dy_stride + sub * V;
-        T* to = p.out + row0 * p.channels + sub * V;
-        Pack<T, V> x_raw[U][K], dy_raw[U][K];
+        const T* x_from = p.x + row0 * p.x_stride;
+        const T* dy_from = p.dy + row0 * p.dy_stride;
+        T* to = p.out + row0 * p.channels;
+        typename Lane::Raw x_raw[U][K], dy_raw[U][K];
         float r[U], mean[U], c1[U], c2[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const bool live = u * rows_per_warp < left;
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const bool in = live && (sub + k * p.lanes) * V < p.channels;
-                x_raw[u][k] = in ? load_pack<T, V>(x_from + u * x_step + k * p.lanes * V) : zero_pack<T, V>();
-                dy_raw[u][k] = in ? load_pack<T, V>(dy_from + u * dy_step + k * p.lanes * V) : zero_pack<T, V>();
+                x_raw[u][k] = live ? columns.load(x_from + u * x_step, k) : zero_pack<T, Lane::kWidth>();
+                dy_raw[u][k] = live ? columns.load(dy_from + u * dy_step, k) : zero_pack<T, Lane::kWidth>();
             }
             r[u] = live ? p.rstd[row0 + u * rows_per_warp] : 0.0f;
             mean[u] = !Rms && live ? p.mean[row0 + u * rows_per_warp] : 0.0f;
@@ -670,7 +705,7 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p, 
             const Pair minus_c1 = both(-count.mean(c1[u])), minus_c2 = both(-count.mean(c2[u]));
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                Pack<T, V> dx;
+                typename Lane::Raw dx;
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
                     const Pair d = get_pair(dy_raw[u][k], i), x = get_pair(x_raw[u][k], i);
@@ -678,13 +713,270 @@ __global__ void __launch_bounds__(kThreads) norm_backward_kernel(NormArgs<T> p, 
                     const Pair g = Rms ? d * w[k][i] : fma(d, w[k][i], minus_c1);
                     set_pair(dx, i, scale * fma(xh, minus_c2, g));
                 }
-                if (u * rows_per_warp < left && (sub + k * p.lanes) * V < p.channels) {
-                    store_pack<T, V>(to + u * down + k * p.lanes * V, dx);
+                if (u * rows_per_warp < left) {
+                    columns.store(to + u * down, k, dx);
                 }
             }
         }
     }
     finish_sums<T, V, K, P>(p, dw, db, sums, dw_out, db_out);
+}
+
+// Rows that lie one behind the other but do not come in 16-byte vectors. A warp takes a batch of
+// them, which is one range of memory: 16-byte copies bring it to shared memory, a lane computes
+// its elements in place there, and 16-byte stores take the batch away; a 16-byte word that two
+// batches share is stored by elements. A batch is on its way while the one before it is computed.
+// 120 MB of rows, forward and backward, against every element loaded from global memory: 62 float16
+// 74 / 120 us (206 / 412), 63 float16 97 / 164 (133 / 176), 191 float16 102 / 173 (144 / 395), 97
+// float32 97 / 130 (98 / 283), 999 float32 88 / 120 (81 / 278). Bound by the instructions that take
+// one or two elements at a time.
+constexpr int kBatchStages = 2;
+constexpr int kBatchBytes = 2560;   // of a batch, at least; 1536 bytes take 62 float16 107 / 177 us
+
+struct Batches {
+    int rows;                     // of a batch
+    int bytes;                    // of its range in shared memory, whatever its start
+    int stage;                    // bytes of a stage: the ranges of x and, backward, dy, rstd and mean
+};
+
+template <typename T> inline Batches batches_of(int channels, int lanes, bool backward) {
+    const int at_once = 32 / lanes, row = channels * static_cast<int>(sizeof(T));
+    Batches b;
+    const int group = at_once * (row + 8);   // with the statistics, which outweigh the narrowest rows
+    b.rows = at_once * ((kBatchBytes + group - 1) / group);
+    b.bytes = (b.rows * row + 15) / 16 * 16 + 16;
+    b.stage = backward ? 2 * b.bytes + (2 * 4 * b.rows + 15) / 16 * 16 : b.bytes;
+    return b;
+}
+
+// blocks of an SM, by the registers that a lane's elements of a row take
+template <int Elements, bool Backward>
+constexpr int kBatchBlocks = Backward ? (Elements <= 4 ? 4 : Elements <= 8 ? 3 : Elements <= 12 ? 2 : 1)
+                                      : (Elements <= 8 ? 4 : Elements <= 12 ? 3 : Elements <= 24 ? 2 : 1);
+
+// A batch of a warp: `row` and the rows behind it, as far as the array goes.
+template <typename T> struct Range {
+    long long begin, end, total;   // bytes of the array
+
+    __device__ __forceinline__ Range(const NormArgs<T>& p, const Batches& b, long long row) {
+        const long long bytes = static_cast<long long>(p.channels) * sizeof(T);
+        total = p.rows * bytes;
+        begin = min(row, p.rows) * bytes;
+        end = min(begin + b.rows * bytes, total);
+    }
+    __device__ __forceinline__ int shift() const { return static_cast<int>(begin & 15); }
+    // 16-byte words that hold a byte of the range, not past the array's end
+    __device__ __forceinline__ void fetch(unsigned char* to, const T* from) const {
+        const long long base = begin - shift();
+        const unsigned char* bytes = reinterpret_cast<const unsigned char*>(from);
+        for (long long at = base + (threadIdx.x & 31) * 16; at < end; at += 512) {
+            const int size = static_cast<int>(min(total - at, 16LL));
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(shared_address(to + (at - base))),
+                         "l"(bytes + at), "r"(size) : "memory");
+        }
+    }
+    __device__ __forceinline__ void store(const unsigned char* from, T* to) const {
+        const int lane = threadIdx.x & 31;
+        const long long base = begin - shift();
+        unsigned char* bytes = reinterpret_cast<unsigned char*>(to);
+        const long long first = min((begin + 15) / 16 * 16, end), last = max(end / 16 * 16, first);
+        for (long long at = first + lane * 16; at < last; at += 512) {
+            *reinterpret_cast<uint4*>(bytes + at) = *reinterpret_cast<const uint4*>(from + (at - base));
+        }
+        // up to 16 / sizeof(T) - 1 elements before the first whole word, and behind the last
+        constexpr int kEdge = 16 / static_cast<int>(sizeof(T));
+        const long long at = lane < kEdge ? begin + lane * static_cast<int>(sizeof(T))
+                                          : last + (lane - kEdge) * static_cast<int>(sizeof(T));
+        if (lane < kEdge ? at < first : lane < 2 * kEdge && at < end) {
+            *reinterpret_cast<T*>(bytes + at) = *reinterpret_cast<const T*>(from + (at - base));
+        }
+    }
+};
+
+template <typename T, int V, int K, bool Rms>
+__global__ void __launch_bounds__(kThreads, kBatchBlocks<Columns<T, V>::kWidth * K, false>) norm_forward_batch_kernel(NormArgs<T> p, Batches batches) {
+    using Lane = Columns<T, V>;
+    constexpr int W = Lane::kWidth, P = W / 2;
+    extern __shared__ __align__(16) unsigned char memory[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sub = lane & (p.lanes - 1), rows_per_warp = 32 / p.lanes;
+    unsigned char* mine = memory + warp * kBatchStages * batches.stage;
+    const Lane columns(sub, p.lanes, p.channels);
+    const Count count(p.channels);
+    Pair w[K][P], b[K][P];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        columns.vector(p.weight, k, 1.0f, w[k]);
+        columns.vector(p.bias, k, 0.0f, b[k]);
+    }
+    const long long step = static_cast<long long>(gridDim.x) * kWarps * batches.rows;
+    long long row = (blockIdx.x * static_cast<long long>(kWarps) + warp) * batches.rows;
+    Range<T>(p, batches, row).fetch(mine, p.x);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    for (int stage = 0; row < p.rows; row += step, stage ^= 1) {
+        Range<T>(p, batches, row + step).fetch(mine + (stage ^ 1) * batches.stage, p.x);
+        asm volatile("cp.async.commit_group;\ncp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        const Range<T> range(p, batches, row);
+        unsigned char* data = mine + stage * batches.stage;
+        const int rows = static_cast<int>(min(p.rows - row, static_cast<long long>(batches.rows)));
+        for (int first = 0; first < rows; first += rows_per_warp) {
+            const int at = first + lane / p.lanes;
+            T* values = reinterpret_cast<T*>(data + range.shift()) + at * p.channels;
+            Pair x[K][P], sum = both(0.0f), squares = both(0.0f);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const auto raw = at < rows ? columns.load(values, k) : zero_pack<T, W>();
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    x[k][i] = get_pair(raw, i);
+                    sum = sum + x[k][i];
+                }
+            }
+            float mean[1] = {0.0f}, r[1];
+            if (!Rms) {
+                mean[0] = sum.x + sum.y;
+                group_sums(mean, p.lanes);
+                mean[0] = count.mean(mean[0]);
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    if (!Rms) {
+                        x[k][i] = columns.within(k, minus(x[k][i], both(mean[0])));
+                    }
+                    squares = fma(x[k][i], x[k][i], squares);
+                }
+            }
+            r[0] = squares.x + squares.y;
+            group_sums(r, p.lanes);
+            r[0] = rsqrtf(fmaf(r[0], count.inverse, p.eps));
+            if (at < rows) {
+                if (sub == 0) {
+                    p.rstd[row + at] = r[0];
+                    if (!Rms) {
+                        p.mean[row + at] = mean[0];
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    typename Lane::Raw y;
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        const Pair xh = x[k][i] * both(r[0]);
+                        set_pair(y, i, Rms ? xh * w[k][i] : fma(xh, w[k][i], b[k][i]));
+                    }
+                    columns.store(values, k, y);
+                }
+            }
+        }
+        __syncwarp();
+        range.store(data, p.out);
+        __syncwarp();   // the next turn's copies overwrite this stage
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+template <typename T, int V, int K, bool Rms>
+__global__ void __launch_bounds__(kThreads, kBatchBlocks<Columns<T, V>::kWidth * K, true>) norm_backward_batch_kernel(
+    NormArgs<T> p, Batches batches, T* dw_out, T* db_out
+) {
+    using Lane = Columns<T, V>;
+    constexpr int W = Lane::kWidth, P = W / 2;
+    extern __shared__ __align__(16) unsigned char memory[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int sub = lane & (p.lanes - 1), rows_per_warp = 32 / p.lanes;
+    unsigned char* mine = memory + warp * kBatchStages * batches.stage;
+    const Lane columns(sub, p.lanes, p.channels);
+    const Count count(p.channels);
+    Pair dw[K][P], db[K][P], w[K][P];
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        columns.vector(p.weight, k, 1.0f, w[k]);
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            dw[k][i] = db[k][i] = both(0.0f);
+        }
+    }
+    const long long step = static_cast<long long>(gridDim.x) * kWarps * batches.rows;
+    long long row = (blockIdx.x * static_cast<long long>(kWarps) + warp) * batches.rows;
+    const auto fetch = [&](long long from, int stage) {
+        const Range<T> range(p, batches, from);
+        unsigned char* data = mine + stage * batches.stage;
+        range.fetch(data, p.x);
+        range.fetch(data + batches.bytes, p.dy);
+        float* stats = reinterpret_cast<float*>(data + 2 * batches.bytes);
+        for (long long i = lane; i < batches.rows && from + i < p.rows; i += 32) {
+            copy_word(stats + i, p.rstd + from + i);
+            if (!Rms) {
+                copy_word(stats + batches.rows + i, p.mean + from + i);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    fetch(row, 0);
+    for (int stage = 0; row < p.rows; row += step, stage ^= 1) {
+        fetch(row + step, stage ^ 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        const Range<T> range(p, batches, row);
+        unsigned char* data = mine + stage * batches.stage;
+        const float* stats = reinterpret_cast<const float*>(data + 2 * batches.bytes);
+        const int rows = static_cast<int>(min(p.rows - row, static_cast<long long>(batches.rows)));
+        for (int first = 0; first < rows; first += rows_per_warp) {
+            const int at = first + lane / p.lanes;
+            const bool live = at < rows;
+            const T* x_values = reinterpret_cast<const T*>(data + range.shift()) + at * p.channels;
+            T* dy_values = reinterpret_cast<T*>(data + batches.bytes + range.shift()) + at * p.channels;
+            const Pair scale = both(live ? stats[at] : 0.0f), shift = both(!Rms && live ? stats[batches.rows + at] : 0.0f);
+            Pair s1 = both(0.0f), s2 = both(0.0f);
+            typename Lane::Raw x_raw[K], dy_raw[K];
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                x_raw[k] = live ? columns.load(x_values, k) : zero_pack<T, W>();
+                dy_raw[k] = live ? columns.load(dy_values, k) : zero_pack<T, W>();
+#pragma unroll
+                for (int i = 0; i < P; ++i) {
+                    const Pair d = get_pair(dy_raw[k], i), x = get_pair(x_raw[k], i);
+                    const Pair xh = (Rms ? x : minus(x, shift)) * scale;
+                    const Pair g = d * w[k][i];
+                    if (!Rms) {
+                        s1 = s1 + g;
+                        db[k][i] = db[k][i] + d;
+                    }
+                    s2 = fma(g, xh, s2);
+                    dw[k][i] = fma(d, xh, dw[k][i]);
+                }
+            }
+            float c1[1] = {s1.x + s1.y}, c2[1] = {s2.x + s2.y};
+            if (!Rms) {
+                group_sums(c1, p.lanes);
+            }
+            group_sums(c2, p.lanes);
+            const Pair minus_c1 = both(-count.mean(c1[0])), minus_c2 = both(-count.mean(c2[0]));
+            if (live) {
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    typename Lane::Raw dx;
+#pragma unroll
+                    for (int i = 0; i < P; ++i) {
+                        const Pair d = get_pair(dy_raw[k], i), x = get_pair(x_raw[k], i);
+                        const Pair xh = (Rms ? x : minus(x, shift)) * scale;
+                        const Pair g = Rms ? d * w[k][i] : fma(d, w[k][i], minus_c1);
+                        set_pair(dx, i, scale * fma(xh, minus_c2, g));
+                    }
+                    columns.store(dy_values, k, dx);
+                }
+            }
+        }
+        __syncwarp();
+        range.store(data + batches.bytes, p.out);
+        __syncwarp();   // the next turn's copies overwrite this stage
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    __syncthreads();   // the batches' memory takes the sums
+    finish_sums<T, V, K, P>(p, dw, db, reinterpret_cast<float*>(memory), dw_out, db_out);
 }
 
 // Rows wider than the registers of a warp: one block per row, three passes over a row that
@@ -828,10 +1120,11 @@ constexpr int kMaxLaneElements = 32;   // values of a row that a lane holds
 constexpr int kMaxNarrow = 32 * kMaxLaneElements;
 
 // Lanes per row and vectors per lane: among the splits that leave the fewest idle slots, the one
-// with the fewest lanes, but not fewer than eight, which read whole 128-byte lines. Fewer lanes
-// take fewer steps to add a row up: 256 float16 channels backward, 120 MB of rows, 107 us with 32
+// with the fewest lanes, but not fewer than `least` (from global memory eight, which read whole
+// 128-byte lines) and with at most `most` vectors each. Fewer lanes take fewer steps to add a row
+// up: 256 float16 channels backward, 120 MB of rows, 107 us with 32
 // lanes, 66 with 16 or 8; 32 float16 channels 66 us with 4 lanes, 79 with 2.
-inline void split_row(int vectors, int elements, int& lanes, int& per_lane) {
+inline void split_row(int vectors, int elements, int least, int most, int& lanes, int& per_lane) {
     long long best_slots = -1;
     for (int l = 32; l >= 1; l >>= 1) {
         const int k = (vectors + l - 1) / l;
@@ -839,7 +1132,7 @@ inline void split_row(int vectors, int elements, int& lanes, int& per_lane) {
             break;
         }
         const long long slots = static_cast<long long>(l) * k;
-        if (best_slots < 0 || slots < best_slots || (slots == best_slots && l >= 8)) {
+        if (best_slots < 0 || slots < best_slots || (slots == best_slots && l >= least && k <= most)) {
             best_slots = slots;
             lanes = l;
             per_lane = k;
@@ -853,13 +1146,26 @@ inline long long blocks_of(long long rows, int lanes, int in_flight) {
 }
 
 template <typename T, int V, int K>
-int launch_forward(const NormArgs<T>& p, bool rms, cudaStream_t stream) {
-    if constexpr (V == 1 || !kForwardRing<T>) {
-        const long long blocks = blocks_of(p.rows, p.lanes, kRowsInFlight<K>);
+int launch_forward(const NormArgs<T>& p, bool rms, bool batches, cudaStream_t stream) {
+    constexpr bool kVectors = V == 16 / static_cast<int>(sizeof(T));
+    if constexpr (!kVectors) {
+        if (batches || V > 1) {
+            const Batches b = batches_of<T>(p.channels, p.lanes, false);
+            const int bytes = kWarps * kBatchStages * b.stage;
+            const long long blocks = std::min<long long>((p.rows - 1) / (kWarps * b.rows) + 1, 148 * 8);
+            auto* kernel = rms ? norm_forward_batch_kernel<T, V, K, true> : norm_forward_batch_kernel<T, V, K, false>;
+            LAT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+            kernel<<<static_cast<unsigned>(blocks), kThreads, bytes, stream>>>(p, b);
+            LAT_LAUNCH_CHECK();
+            return LAT_OK;
+        }
+    }
+    if constexpr (V == 1 || (kVectors && !kForwardRing<T>)) {
+        const long long blocks = blocks_of(p.rows, p.lanes, kRowsInFlight<Columns<T, V>::kWidth * K * sizeof(T)>);
         LAT_REQUIRE(blocks <= 0x7fffffffLL, "normalisation supports at most 2^31 blocks of rows.");
         auto* kernel = rms ? norm_forward_kernel<T, V, K, true> : norm_forward_kernel<T, V, K, false>;
         kernel<<<static_cast<unsigned>(blocks), kThreads, 0, stream>>>(p);
-    } else {
+    } else if constexpr (kVectors) {
         constexpr int kBytes = kForwardStages<K> * kForwardRows<K> * K * kThreads * 16;
         const long long blocks = std::min<long long>(blocks_of(p.rows, p.lanes, kForwardRows<K>), 148 * kForwardBlocks<V, K>);
         auto* kernel = rms ? norm_forward_ring_kernel<T, K, true> : norm_forward_ring_kernel<T, K, false>;
@@ -870,7 +1176,7 @@ int launch_forward(const NormArgs<T>& p, bool rms, cudaStream_t stream) {
     return LAT_OK;
 }
 
-constexpr int kMaxBackwardBlocks = 148 * 3;
+constexpr int kMaxBackwardBlocks = 148 * 4;
 constexpr int kMaxChannels = 65535 * kThreads;   // of the sums' grid
 
 template <typename T> int launch_reduce(const NormArgs<T>& p, int blocks, T* dw, T* db, cudaStream_t stream) {
@@ -881,17 +1187,31 @@ template <typename T> int launch_reduce(const NormArgs<T>& p, int blocks, T* dw,
 }
 
 template <typename T, int V, int K>
-int launch_backward(const NormArgs<T>& p, bool rms, T* dw, T* db, cudaStream_t stream) {
+int launch_backward(const NormArgs<T>& p, bool rms, bool batches, T* dw, T* db, cudaStream_t stream) {
     const size_t sums = sizeof(float) * kWarps * p.channels;
-    int grid;
+    int grid = 1;
+    constexpr bool kVectors = V == 16 / static_cast<int>(sizeof(T));
+    if constexpr (!kVectors) {
+        if (batches || V > 1) {
+            const Batches b = batches_of<T>(p.channels, p.lanes, true);
+            const size_t smem = std::max<size_t>(kWarps * kBatchStages * b.stage, sums);
+            grid = static_cast<int>(std::min<long long>((p.rows - 1) / (kWarps * b.rows) + 1, kMaxBackwardBlocks));
+            auto* kernel = rms ? norm_backward_batch_kernel<T, V, K, true> : norm_backward_batch_kernel<T, V, K, false>;
+            LAT_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+            kernel<<<grid, kThreads, smem, stream>>>(p, b, dw, db);
+            LAT_LAUNCH_CHECK();
+            return grid > 1 && (dw != nullptr || db != nullptr) ? launch_reduce(p, grid, dw, db, stream) : LAT_OK;
+        }
+    }
     if constexpr (V == 1) {
-        grid = static_cast<int>(std::min<long long>(blocks_of(p.rows, p.lanes, kPlainRows<K>), 148 * 2));
+        constexpr int kRows = kBackwardRows<Columns<T, V>::kWidth * K * sizeof(T)>;
+        grid = static_cast<int>(std::min<long long>(blocks_of(p.rows, p.lanes, kRows), kMaxBackwardBlocks));
         if (rms) {
             norm_backward_kernel<T, K, true><<<grid, kThreads, sums, stream>>>(p, dw, db);
         } else {
             norm_backward_kernel<T, K, false><<<grid, kThreads, sums, stream>>>(p, dw, db);
         }
-    } else {
+    } else if constexpr (kVectors) {
         grid = static_cast<int>(std::min<long long>(blocks_of(p.rows, p.lanes, kRingRows<K>), 148 * kRingBlocks<V, K>));
         const size_t smem = std::max(ring_bytes<K>(), sums);
         auto* kernel = rms ? norm_backward_ring_kernel<T, K, true> : norm_backward_ring_kernel<T, K, false>;
@@ -903,17 +1223,17 @@ int launch_backward(const NormArgs<T>& p, bool rms, T* dw, T* db, cudaStream_t s
 }
 
 template <typename T, int V, bool Backward>
-int dispatch_split(NormArgs<T> p, bool rms, T* dw, T* db, cudaStream_t stream) {
-    constexpr int kMost = kMaxLaneElements / V;
+int dispatch_split(NormArgs<T> p, bool rms, bool batches, T* dw, T* db, cudaStream_t stream) {
+    constexpr int kWidth = Columns<T, V>::kWidth, kMost = kMaxLaneElements / kWidth;
     int k;
-    split_row(p.channels / V, V, p.lanes, k);
+    split_row((p.channels + kWidth - 1) / kWidth, kWidth, batches ? 1 : 8, batches ? 8 / kWidth : kMost, p.lanes, k);
 #define LAT_NORM_CASE(N)                                                            \
     if constexpr (N <= kMost) {                                                     \
         if (k <= N) {                                                               \
             if constexpr (Backward) {                                               \
-                return launch_backward<T, V, N>(p, rms, dw, db, stream);            \
+                return launch_backward<T, V, N>(p, rms, batches, dw, db, stream);   \
             } else {                                                                \
-                return launch_forward<T, V, N>(p, rms, stream);                     \
+                return launch_forward<T, V, N>(p, rms, batches, stream);            \
             }                                                                       \
         }                                                                           \
     }
@@ -923,16 +1243,35 @@ int dispatch_split(NormArgs<T> p, bool rms, T* dw, T* db, cudaStream_t stream) {
     LAT_NORM_CASE(4)
     LAT_NORM_CASE(6)
     LAT_NORM_CASE(8)
+    LAT_NORM_CASE(12)
     LAT_NORM_CASE(16)
-    LAT_NORM_CASE(32)
 #undef LAT_NORM_CASE
     return fail(LAT_INVALID_ARGUMENT, "unsupported channel count.");
 }
 
-template <typename T> bool vector_rows(const NormArgs<T>& p) {
-    constexpr int V = 16 / sizeof(T);
-    return p.channels % V == 0 && p.x_stride % V == 0 && p.dy_stride % V == 0 && aligned_to(p.x, 16) &&
-           aligned_to(p.dy, 16) && aligned_to(p.out, 16) && aligned_to(p.weight, 16) && aligned_to(p.bias, 16);
+// Rows of 16-byte vectors; others one behind the other in batches; the rest by elements.
+template <typename T, bool Backward>
+int dispatch(const NormArgs<T>& p, bool rms, T* dw, T* db, cudaStream_t stream) {
+    constexpr int V = 16 / static_cast<int>(sizeof(T));
+    const bool aligned = aligned_to(p.x, 16) && aligned_to(p.dy, 16) && aligned_to(p.out, 16);
+    if (aligned && p.channels % V == 0 && p.x_stride % V == 0 && p.dy_stride % V == 0 && aligned_to(p.weight, 16) &&
+        aligned_to(p.bias, 16)) {
+        return dispatch_split<T, V, Backward>(p, rms, false, dw, db, stream);
+    }
+    if (!aligned || p.x_stride != p.channels || (Backward && p.dy_stride != p.channels)) {
+        return dispatch_split<T, 1, Backward>(p, rms, false, dw, db, stream);
+    }
+    // the widest vectors that rows, weight and bias come in
+    const auto fits = [&](int v) {
+        return p.channels % v == 0 && aligned_to(p.weight, v * sizeof(T)) && aligned_to(p.bias, v * sizeof(T));
+    };
+    if constexpr (V == 8) {
+        if (fits(4)) {
+            return dispatch_split<T, 4, Backward>(p, rms, true, dw, db, stream);
+        }
+    }
+    return fits(2) ? dispatch_split<T, 2, Backward>(p, rms, true, dw, db, stream)
+                   : dispatch_split<T, 1, Backward>(p, rms, true, dw, db, stream);
 }
 
 template <typename T> int run_forward(const NormArgs<T>& p, bool rms, cudaStream_t stream) {
@@ -946,8 +1285,7 @@ template <typename T> int run_forward(const NormArgs<T>& p, bool rms, cudaStream
         LAT_LAUNCH_CHECK();
         return LAT_OK;
     }
-    return vector_rows(p) ? dispatch_split<T, 16 / sizeof(T), false>(p, rms, nullptr, nullptr, stream)
-                          : dispatch_split<T, 1, false>(p, rms, nullptr, nullptr, stream);
+    return dispatch<T, false>(p, rms, nullptr, nullptr, stream);
 }
 
 // Partial rows that the backward pass may write.
@@ -958,8 +1296,7 @@ inline int partial_rows(long long rows) {
 template <typename T>
 int run_backward(const NormArgs<T>& p, bool rms, T* dw, T* db, cudaStream_t stream) {
     if (p.channels <= kMaxNarrow) {
-        return vector_rows(p) ? dispatch_split<T, 16 / sizeof(T), true>(p, rms, dw, db, stream)
-                              : dispatch_split<T, 1, true>(p, rms, dw, db, stream);
+        return dispatch<T, true>(p, rms, dw, db, stream);
     }
     const int grid = static_cast<int>(std::min(p.rows, 148LL * 8));
     if (rms) {

@@ -105,6 +105,68 @@ def test_row_norm_values_and_gradients(cuda, dtype, rms, rows, channels):
 
 
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('rms', [False, True])
+@pytest.mark.parametrize('rows,channels', [
+    (9001, 3), (7003, 5), (6001, 21), (5003, 60), (5001, 62), (5000, 63), (2100, 130), (2003, 191), (901, 300),
+    (700, 513), (401, 766), (301, 999), (1, 999), (2, 1023), (9, 1022),
+])
+def test_row_norm_of_rows_that_are_no_vectors(cuda, dtype, rms, rows, channels):
+    """Rows of every width modulo 16 bytes, several batches a warp and a ragged last one; what
+    lies behind the arrays stays as it was."""
+    from mlx_lattice_b200 import _ext
+
+    rng = np.random.default_rng(rows + channels)
+    x = _randn(rng, rows, channels, dtype=dtype, scale=2.0, shift=1.0)
+    dy = _randn(rng, rows, channels, dtype=dtype)
+    weight = _randn(rng, channels, dtype=dtype, shift=1.0)
+    bias = None if rms else _randn(rng, channels, dtype=dtype)
+    want = _norm_reference(_np(x), _np(weight), None if rms else _np(bias), _np(dy), 1e-3, rms)
+    y, mean, rstd = _ext.row_norm_forward(x, weight, bias, 1e-3, rms)
+    dx, dw, db = _ext.row_norm_backward(dy, x, weight, mean, rstd, rms, True, not rms)
+    for got, name in ((y, 'y'), (dx, 'dx'), (dw, 'dw'), (db, 'db')):
+        if got is not None:
+            _close(got, *want[name], dtype, name)
+    again, *stats = _ext.row_norm_forward(x, weight, bias, 1e-3, rms)
+    assert torch.equal(y, again)
+    assert all(torch.equal(a, b) for a, b in zip(
+        (dx, dw), _ext.row_norm_backward(dy, x, weight, mean, rstd, rms, True, not rms)))
+    # the same rows in a wider array, element by element
+    wide = torch.zeros((rows, channels + 1), dtype=dtype, device=cuda)
+    wide[:, :channels] = x
+    y, mean, rstd = _ext.row_norm_forward(wide[:, :channels], weight, bias, 1e-3, rms)
+    _close(y, *want['y'], dtype, 'y')
+    dx, dw, db = _ext.row_norm_backward(dy, wide[:, :channels], weight, mean, rstd, rms, True, not rms)
+    for got, name in ((dx, 'dx'), (dw, 'dw'), (db, 'db')):
+        if got is not None:
+            _close(got, *want[name], dtype, name)
+
+
+@pytest.mark.parametrize('rms', [0, 1])
+@pytest.mark.parametrize('channels', [5, 63, 62, 999])
+def test_row_norm_writes_its_rows_only(cuda, rms, channels):
+    """Outputs in the middle of a buffer: the bytes around them stay."""
+    from mlx_lattice_b200 import _native
+
+    lib = _native.load()
+    rows, pad = 37, 64
+    x = torch.randn(rows, channels, device=cuda).half()
+    ptr = lambda t: None if t is None else t.data_ptr()
+    buffers = [torch.full((rows * channels + 2 * pad,), 7.0, device=cuda, dtype=torch.float16) for _ in range(2)]
+    stats = [torch.full((rows + 2 * pad,), 7.0, device=cuda) for _ in range(2)]
+    y, dx = (b[pad:pad + rows * channels] for b in buffers)
+    mean, rstd = (s[pad:pad + rows] for s in stats)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.lat_row_norm_forward(1, rms, ptr(x), rows, channels, channels, None, None, 1e-5, ptr(y),
+                                    None if rms else ptr(mean), ptr(rstd), stream) == _native.LAT_OK
+    assert lib.lat_row_norm_backward(1, rms, ptr(x), channels, ptr(x), rows, channels, channels, None,
+                                     None if rms else ptr(mean), ptr(rstd), ptr(dx), None, None, None, 0,
+                                     stream) == _native.LAT_OK
+    for buffer in (*buffers, *stats):
+        assert (buffer[:pad] == 7).all() and (buffer[-pad:] == 7).all()
+    assert (y.view(rows, channels).float() - x.float()).abs().max() > 0 and not (dx == 7).all()
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
 def test_row_norm_strided_and_unaligned_rows(cuda, dtype):
     """Columns of a wider array, rows that start off a 16-byte boundary, a broadcast gradient,
     no weight, and only some of the gradients asked for."""
