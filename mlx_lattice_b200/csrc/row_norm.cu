@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, K <= 6 ? 2 : 1) norm_backward_kernel
 // float32 97 / 130 (98 / 283), 999 float32 88 / 120 (81 / 278). Bound by the instructions that take
 // one or two elements at a time.
 constexpr int kBatchStages = 2;
-constexpr int kBatchBytes = 2560;   // of a batch, at least; 1536 bytes take 62 float16 107 / 177 us
+constexpr int kBatchBytes = 2560;   // of a batch, at least; 1536 bytes take 63 float16 105 / 175 us
 
 struct Batches {
     int rows;                     // of a batch

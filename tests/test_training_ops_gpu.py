@@ -491,6 +491,53 @@ def test_recurrence_ragged_sequences(cuda, dtype, reverse, channels):
     _check_recurrence(cuda, dtype, 731, channels, offsets, reverse, initial=True)
 
 
+@pytest.mark.parametrize('reverse', [False, True])
+@pytest.mark.parametrize('channels', [5, 7, 9, 63, 129, 513])
+def test_recurrence_of_odd_widths(cuda, channels, reverse):
+    """float16 rows whose starts fall on both halves of a four-byte word."""
+    _check_recurrence(cuda, torch.float16, 300, channels, [0, 9, 150, 150, 270], reverse, True, seed=channels)
+
+
+@pytest.mark.parametrize('reverse', [0, 1])
+@pytest.mark.parametrize('channels,start', [(7, 0), (7, 1), (64, 1), (13, 3)])
+def test_recurrence_writes_its_rows_only(cuda, channels, start, reverse):
+    """Inputs and outputs at any element of a buffer: values as from the start of one, and the
+    elements around the outputs stay."""
+    from mlx_lattice_b200 import _ext, _native
+
+    lib = _native.load()
+    rows, pad = 75, 64
+    rng = np.random.default_rng(channels)
+    off = torch.tensor([0, 20, 75], dtype=torch.int32, device=cuda)
+
+    def placed(t=None):
+        buffer = torch.full((rows * channels + 2 * pad,), 7.0, device=cuda, dtype=torch.float16)
+        view = buffer[pad + start:pad + start + rows * channels].view(rows, channels)
+        if t is not None:
+            view.copy_(t)
+        return buffer, view
+
+    x, z, dy = (_randn(rng, rows, channels, dtype=torch.float16) for _ in range(3))
+    h, _, carries = _ext.recurrence_forward(x, z, off, None, bool(reverse), want_carries=True)
+    dx, dz, _ = _ext.recurrence_backward(dy, None, x, z, off, None, bool(reverse), carries)
+    kept = [placed(t) for t in (x, z, dy)]
+    xp, zp, dyp = (view.data_ptr() for _, view in kept)
+    outs = [placed() for _ in range(3)]
+    need = lib.lat_recurrence_workspace_bytes(1, rows, channels)
+    workspace = torch.empty(need, dtype=torch.uint8, device=cuda)
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.lat_recurrence_forward(
+        1, xp, channels, zp, channels, rows, channels, off.data_ptr(), 2, None, reverse, outs[0][1].data_ptr(), None,
+        carries.data_ptr(), workspace.data_ptr(), need, None, stream) == _native.LAT_OK
+    assert lib.lat_recurrence_backward(
+        1, dyp, channels, None, xp, channels, zp, channels, rows, channels, off.data_ptr(), 2, None, reverse,
+        carries.data_ptr(), outs[1][1].data_ptr(), outs[2][1].data_ptr(), None, workspace.data_ptr(), need, None,
+        stream) == _native.LAT_OK
+    for (buffer, view), want in zip(outs, (h, dx, dz)):
+        assert torch.equal(view, want)
+        assert (buffer[:pad + start] == 7).all() and (buffer[pad + start + rows * channels:] == 7).all()
+
+
 @pytest.mark.parametrize('dtype', DTYPES)
 @pytest.mark.parametrize('rows,offsets', [
     (1, [0, 1]), (1, [0, 0]), (7, [0, 7]), (127, [0, 127]), (128, [0, 128]), (129, [0, 129]), (2049, [0, 2049]),
