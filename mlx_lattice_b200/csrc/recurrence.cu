@@ -260,7 +260,7 @@ template <typename T, int N, int Granule> struct Channels {
     static constexpr int kBytes = N * static_cast<int>(sizeof(T));
     static constexpr int kMove = Granule < kBytes ? Granule : kBytes;
     static constexpr bool kShifted = Granule == 2;
-    [[maybe_unused]] static constexpr int kMoveChannels = kMove / static_cast<int>(sizeof(T));
+    static constexpr int kMoveChannels = kMove / static_cast<int>(sizeof(T));
     int c, count;
     int lane, live;       // this thread and how many of the tile's threads have channels
     long long row_step;   // from a row to the next one, in rows of an array
@@ -367,7 +367,7 @@ template <typename T, int N, int Granule> struct Channels {
 
     // the thread's channels are whole quads of floats there
     static __device__ __forceinline__ bool quads(const float* at, int channels) {
-        return kMove == kBytes && N % 4 == 0 && channels % 4 == 0 && reinterpret_cast<uintptr_t>(at) % 16 == 0;
+        return kMoveChannels == N && N % 4 == 0 && channels % 4 == 0 && reinterpret_cast<uintptr_t>(at) % 16 == 0;
     }
 
     __device__ __forceinline__ void store_state(float* to, long long row, int channels, const Row<N>& value) const {
