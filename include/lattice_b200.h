@@ -474,7 +474,7 @@ int lat_row_norm(
 
 /* The same normalisation for training (no counterpart in the reference's native extension:
  * its array library differentiates layer_norm / rms_norm). Rows of `feats` are
- * feat_row_stride elements apart, `out` is dense. Leaves the row statistics in float32: mean
+ * feat_row_stride elements apart, `out` is dense; at most 16776960 channels. Leaves the row statistics in float32: mean
  * [rows] (layer norm only, else NULL) and rstd [rows] = 1 / sqrt(variance + eps). */
 int lat_row_norm_forward(
     int32_t dtype, int32_t rms, const void* feats, int64_t rows, int32_t channels, int64_t feat_row_stride,
@@ -511,7 +511,7 @@ int lat_dropout(
  * is dense; final_state [sequences, channels] float32 (or NULL) is the h after the last row (an
  * empty sequence hands its initial state on). carries (NULL unless a backward pass follows):
  * float32 [lat_recurrence_carry_rows(rows), channels], the h before every eighth row. Bitwise
- * repeatable. */
+ * repeatable. At most 2097120 channels. */
 size_t lat_recurrence_workspace_bytes(int32_t dtype, int32_t rows, int32_t channels);
 int32_t lat_recurrence_carry_rows(int32_t rows);
 int lat_recurrence_forward(
@@ -533,7 +533,7 @@ int lat_recurrence_backward(
 
 /* One row of every stream: next_state = a state + (1 - a) x with a = sigmoid(gate), `out` the
  * same rounded to the feature type. state and next_state [rows, channels] float32; next_state
- * may be state itself. */
+ * may be state itself, or lies apart from all inputs. */
 int lat_recurrence_step(
     int32_t dtype, const void* feats, int64_t feat_row_stride, const void* gate, int64_t gate_row_stride,
     const float* state, int64_t rows, int32_t channels, void* out, float* next_state, void* stream);

@@ -14,7 +14,7 @@
 // Both are bound by the memory, or nearly so (a copy moves 6.55 TB/s):
 //   960,000 x 64 float16, layer   forward 41 us, 5.9 TB/s   backward 64 us + sums 3 us, 5.7 TB/s
 //   240,001 x 192 float16, RMS    forward 28 us, 6.5 TB/s   backward 49 us + sums 3 us, 5.6 TB/s
-//   30,011 x 1000 float32, layer  forward 40 us, 6.0 TB/s   backward 61 us + sums 3 us, 5.9 TB/s
+//   30,011 x 1000 float32, layer  forward 43 us, 5.6 TB/s   backward 61 us + sums 3 us, 5.9 TB/s
 // What the backward pass of narrow rows still loses is instructions: two shuffle trees a row and
 // the sums down the rows.
 //
@@ -103,18 +103,22 @@ template <typename T, int V> struct Columns {
     }
     // a step of a vector of the row's length, or `value` without one
     __device__ __forceinline__ void vector(const T* from, int k, float value, Pair (&to)[kWidth / 2]) const {
-        Raw raw = zero_pack<T, kWidth>();
         if (from != nullptr) {
-            raw = load(from, k);
-        }
+            const Raw raw = load(from, k);
 #pragma unroll
-        for (int i = 0; i < kWidth / 2; ++i) {
-            to[i] = from != nullptr ? get_pair(raw, i) : both(value);
+            for (int i = 0; i < kWidth / 2; ++i) {
+                to[i] = get_pair(raw, i);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < kWidth / 2; ++i) {
+                to[i] = both(value);
+            }
         }
     }
-    // a step with zeros behind the row's end
+    // a pair of a step that the row has, with a zero behind the row's end
     __device__ __forceinline__ Pair within(int k, Pair value) const {
-        return {has(k) ? value.x : 0.0f, (V == 1 ? has(k, 1) : has(k)) ? value.y : 0.0f};
+        return {value.x, V > 1 || has(k, 1) ? value.y : 0.0f};
     }
 };
 
@@ -195,12 +199,14 @@ __global__ void __launch_bounds__(kThreads) norm_forward_kernel(NormArgs<T> p) {
         Pair squares = both(0.0f);
 #pragma unroll
         for (int k = 0; k < K; ++k) {
+            if (columns.has(k)) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                if (!Rms) {
-                    x[u][k][i] = columns.within(k, minus(x[u][k][i], both(mean[u])));
+                for (int i = 0; i < P; ++i) {
+                    if (!Rms) {
+                        x[u][k][i] = columns.within(k, minus(x[u][k][i], both(mean[u])));
+                    }
+                    squares = fma(x[u][k][i], x[u][k][i], squares);
                 }
-                squares = fma(x[u][k][i], x[u][k][i], squares);
             }
         }
         r[u] = squares.x + squares.y;
@@ -841,12 +847,14 @@ __global__ void __launch_bounds__(kThreads, kBatchBlocks<Columns<T, V>::kWidth *
             }
 #pragma unroll
             for (int k = 0; k < K; ++k) {
+                if (columns.has(k)) {
 #pragma unroll
-                for (int i = 0; i < P; ++i) {
-                    if (!Rms) {
-                        x[k][i] = columns.within(k, minus(x[k][i], both(mean[0])));
+                    for (int i = 0; i < P; ++i) {
+                        if (!Rms) {
+                            x[k][i] = columns.within(k, minus(x[k][i], both(mean[0])));
+                        }
+                        squares = fma(x[k][i], x[k][i], squares);
                     }
-                    squares = fma(x[k][i], x[k][i], squares);
                 }
             }
             r[0] = squares.x + squares.y;

@@ -141,6 +141,31 @@ def test_row_norm_of_rows_that_are_no_vectors(cuda, dtype, rms, rows, channels):
             _close(got, *want[name], dtype, name)
 
 
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('channels', [64, 60, 63])
+def test_row_norm_of_arrays_off_a_boundary(cuda, dtype, channels):
+    """Rows, or only weight and bias, that start at an odd element of their buffers."""
+    from mlx_lattice_b200 import _ext
+
+    rng = np.random.default_rng(channels)
+    rows = 700
+    x, dy = _randn(rng, rows, channels, dtype=dtype), _randn(rng, rows, channels, dtype=dtype)
+    weight, bias = _randn(rng, channels, dtype=dtype, shift=1.0), _randn(rng, channels, dtype=dtype)
+    want = _norm_reference(_np(x), _np(weight), _np(bias), _np(dy), 1e-3, False)
+
+    def off(t):
+        buffer = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+        buffer[1:] = t.flatten()
+        return buffer[1:].view(t.shape)
+
+    for args in ((x, off(weight), off(bias), dy), (off(x), weight, bias, dy), (x, weight, bias, off(dy)),
+                 (off(x), off(weight), bias, off(dy))):
+        y, mean, rstd = _ext.row_norm_forward(*args[:3], 1e-3, False)
+        grads = _ext.row_norm_backward(args[3], args[0], args[1], mean, rstd, False, True, True)
+        for got, name in zip((y, *grads), ('y', 'dx', 'dw', 'db')):
+            _close(got, *want[name], dtype, name)
+
+
 @pytest.mark.parametrize('rms', [0, 1])
 @pytest.mark.parametrize('channels', [5, 63, 62, 999])
 def test_row_norm_writes_its_rows_only(cuda, rms, channels):
@@ -717,6 +742,30 @@ def test_recurrence_step_into_a_given_state(cuda):
     ops.gated_recurrence_step(_sparse(feats[:1]), feats[:1], state, out_state=state)
     with pytest.raises(RuntimeError, match='modified by an inplace operation'):
         y.sum().backward()
+
+
+def test_many_sequences_without_rows_hand_their_state_on(cuda):
+    """More empty sequences than a warp has threads, at both ends and between rows."""
+    from mlx_lattice_b200 import _ext
+
+    rng = np.random.default_rng(60)
+    for channels in (3, 40):
+        cuts = [4] * 90 + [30] * 70 + [31, 75] + [75] * 41
+        x, z, dy = (_randn(rng, 80, channels) for _ in range(3))
+        off = torch.tensor(cuts, dtype=torch.int32, device=cuda)
+        initial = _randn(rng, len(cuts) - 1, channels)
+        for reverse in (False, True):
+            h, final, carries = _ext.recurrence_forward(x, z, off, initial, reverse, want_state=True, want_carries=True)
+            dfinal = _randn(rng, len(cuts) - 1, channels)
+            _, _, dinitial = _ext.recurrence_backward(dy, dfinal, x, z, off, initial, reverse, carries, want_initial=True)
+            empty = (off[1:] == off[:-1]).nonzero().flatten()
+            assert len(empty) == len(cuts) - 1 - 3
+            assert torch.equal(final[empty], initial[empty]) and torch.equal(dinitial[empty], dfinal[empty])
+            ref = _recurrence_reference(_np(x), _np(z), cuts, _np(initial), reverse, _np(dy), _np(dfinal))
+            _close(h, *ref['h'], torch.float32, 'h')
+            _close(final, *ref['final'], torch.float32, 'final')
+            _close(dinitial, *ref['dinitial'], torch.float32, 'dinitial')
+    _ext.check_status(cuda)
 
 
 def test_prefill_then_steps(cuda):
