@@ -446,7 +446,8 @@ template <typename T, int N, int Granule, int Arrays, int Rows, int Stages, int 
         for (int r = 0; r < Rows; ++r) {
             if (rows >= Rows || r < rows) {
                 if constexpr (Lanes::kShifted) {
-                    // bytes from the first channel's word on; no byte behind the last channel is read
+                    // Bytes from the first channel's word on: no byte behind the last channel is read, and
+                    // the two before the first one, if any, share its aligned word.
                     const int skip = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 2);
                     const int bytes = skip + lanes.count * static_cast<int>(sizeof(T));
                     const unsigned char* words = reinterpret_cast<const unsigned char*>(at) - skip;
