@@ -116,14 +116,22 @@ bool wants_gradient(std::initializer_list<Tensor> tensors) {
 OptionalTensor none_if_undefined(const Tensor& t) { return t.defined() ? OptionalTensor(t) : std::nullopt; }
 Tensor plain(const OptionalTensor& t) { return t.value_or(Tensor()); }
 
-// The backward passes are not differentiable themselves: their results say so when someone tries.
-variable_list once(variable_list grads) {
-    if (at::GradMode::is_enabled()) {
-        const auto node = std::make_shared<torch::autograd::DelayedError>(
-            "this operator has no second derivative", static_cast<int64_t>(grads.size()));
-        return (*node)(std::move(grads));
+// The same values behind a node that raises `message` when someone differentiates through them. The
+// node attaches itself only to what requires a gradient, so every tensor enters it as one that does.
+variable_list raising(variable_list values, const char* message) {
+    for (Tensor& t : values) {
+        if (t.defined()) {
+            t = t.detach().requires_grad_(true);
+        }
     }
-    return grads;
+    const auto node = std::make_shared<torch::autograd::DelayedError>(message, static_cast<int64_t>(values.size()));
+    return (*node)(std::move(values));
+}
+
+// The backward passes are not differentiable themselves: with a graph of them asked for, their
+// results say so when someone tries.
+variable_list once(variable_list grads) {
+    return at::GradMode::is_enabled() ? raising(std::move(grads), "this operator has no second derivative") : grads;
 }
 
 // ---- row normalisation ------------------------------------------------------------------------
