@@ -7,6 +7,10 @@
 //   dh_t = dy_t + a_{t+1} dh_{t+1}  (+ dfinal at the last row)
 //   dx_t = (1 - a_t) dh_t,  dz_t = a_t (1 - a_t) dh_t (h_{t-1} - x_t),  dinitial = a_1 dh_1
 //
+// Both a_t and 1 - a_t are computed to full relative precision, so a nearly closed gate lets in what
+// it should, and so are A and 1 - A of the maps below, so a long memory does not gather the rounding
+// of gates near one.
+//
 // Both directions are scans over affine maps h -> A h + H, which compose associatively. The
 // rows are cut into tiles of 32. Three kernels:
 //   maps:   for a group of tiles (a block, 128 rows of 128 bytes) the map (A, H) of the group and,
@@ -18,8 +22,9 @@
 // bitwise repeatable.
 //
 // A row that starts a sequence cuts the chain. Its map ignores the incoming h altogether
-// (marked by A = -1, and selected, not multiplied by zero: a NaN or an infinity of one
-// sequence does not reach the next). Rows outside all sequences give zeros.
+// (marked, and selected, not multiplied by zero: a NaN or an infinity of one sequence does not
+// reach the next). Within a sequence an infinite h stays infinite. Rows outside all sequences
+// give zeros.
 //
 // The backward pass recomputes h from the state at the start of every eight rows, which the
 // forward pass leaves in float32: it reads x, z, dy and writes dx, dz, and its h is not rounded
@@ -42,21 +47,60 @@ constexpr int kThreads = 256;                 // of the others
 constexpr int kWindow = 64;                   // groups
 constexpr int kMapBytes = 16;                 // channels of a thread of the maps and apply kernels
 constexpr int kGradientBytes = 8;             // of the gradient kernel, which keeps twice as much of each
-constexpr float kReset = -1.0f;
 constexpr int kScanChannels = 32;             // of a block of the scan kernel
 constexpr int kCarryRows = 8;                 // rows from one kept state to the next
 
-// later after earlier, as maps
-__device__ __forceinline__ float2 compose(float2 earlier, float2 later) {
-    if (later.x == kReset) {
-        return later;
-    }
-    return make_float2(earlier.x == kReset ? kReset : later.x * earlier.x, fmaf(later.x, earlier.y, later.y));
+// ---- maps ----------------------------------------------------------------------------------
+//
+// A map h -> A h + H is kept as the pair (m, H). Of A and 1 - A, m holds the one that is at most one
+// half: A itself, or -(1 - A), told apart by the sign bit. Both are then known to full relative
+// precision. A = 1 - 2^-14 alone would give 1 - A to 2^-11 of itself, and a memory of 2^14 rows h
+// no better.
+constexpr float kReset = 2.0f;   // m of a map that ignores what comes in
+
+__device__ __forceinline__ bool negative(float v) { return __float_as_int(v) < 0; }
+__device__ __forceinline__ bool finite(float v) { return fabsf(v) < __int_as_float(0x7f800000); }
+
+__device__ __forceinline__ float2 make_map(float keep, float rest, float sum, bool cut) {
+    const float m = keep <= 0.5f ? keep : -rest;
+    return make_float2(cut ? kReset : m, sum);
+}
+__device__ __forceinline__ float2 identity() { return make_map(1.0f, 0.0f, 0.0f, false); }
+
+// A near one moves h by 1 - A of it, so that a chain of maps does not gather the rounding of A. An
+// infinity stays, also where A has become zero.
+__device__ __forceinline__ float apply(float2 map, float h) {
+    const float moved = __fadd_rn(fmaf(map.x, h, map.y), negative(map.x) ? h : 0.0f);
+    const float any = finite(h) ? moved : h + map.y;
+    return map.x == kReset ? map.y : any;
 }
 
-__device__ __forceinline__ float apply(float2 map, float h) {
-    return map.x == kReset ? map.y : fmaf(map.x, h, map.y);
-}
+// Maps, one after the other: A, 1 - A and H of them all. What a later map rounds is relative to the H
+// of the ones before it alone. (The products and sums are written as such: a multiply-add that the
+// compiler makes of some of them would let results depend on the launch.)
+struct Chain {
+    float keep = 1.0f, rest = 0.0f, sum = 0.0f;
+    bool cut = false;
+
+    __device__ __forceinline__ void add(const Chain& later) {
+        rest = fmaf(keep, later.rest, rest);
+        keep = __fmul_rn(keep, later.keep);
+        const float moved = fmaf(later.keep, sum, later.sum), any = finite(sum) ? moved : __fadd_rn(sum, later.sum);
+        sum = later.cut ? later.sum : any;
+        cut = cut | later.cut;
+    }
+    __device__ __forceinline__ void add(float2 later) {
+        const bool close = negative(later.x);
+        const float plus = __fadd_rn(1.0f, later.x), less = __fsub_rn(1.0f, later.x);
+        add(Chain{close ? plus : later.x, close ? -later.x : less, later.y, later.x == kReset});
+    }
+    __device__ __forceinline__ float2 map() const { return make_map(keep, rest, sum, cut); }
+    template <typename Later> __device__ __forceinline__ float2 then(const Later& later) const {
+        Chain both = *this;
+        both.add(later);
+        return both.map();
+    }
+};
 
 // Rows and sequences in the order of time: row i is row rows - 1 - i of the arrays when the
 // recurrence runs backwards, and sequence j is sequence sequences - 1 - j.
@@ -87,28 +131,36 @@ __device__ __forceinline__ float reciprocal(float v) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
     return r;
 }
-__device__ __forceinline__ float max_or_nan(float a, float b) {
+__device__ __forceinline__ float min_or_nan(float a, float b) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
     return r;
 }
 
 constexpr float kMinusLog2E = -1.4426950408889634f;
+constexpr float kTiny = 1.1754943508222875e-38f;   // 2^-126
 
-// exp(-z). sigmoid(z) = 1 / (1 + exp(-z)) and sigmoid(-z) = exp(-z) sigmoid(z), each to full
-// relative precision as long as exp(-z) stays below 2^126, where the reciprocal becomes zero.
-// That is z > -87.336; below, sigmoid(z) is less than the smallest normal float anyway.
-constexpr float kLowestGate = -87.33f;
-
-__device__ __forceinline__ Pair exp_minus(Pair z) {
+// exp(-z), at most 2^126. The product with log2(e) is rounded once before the exponential, so it is
+// off by up to (1.25 |z| + 4) 2^-24 of itself. Zero for z > 87.3.
+__device__ __forceinline__ Pair odds_of(Pair z) {
     const Pair t = z * both(kMinusLog2E);
-    return {exp2_fast(t.x), exp2_fast(t.y)};
+    return {min_or_nan(exp2_fast(t.x), 1.0f / kTiny), min_or_nan(exp2_fast(t.y), 1.0f / kTiny)};
 }
-__device__ __forceinline__ Pair sigmoid_from(Pair odds) {
-    const Pair d = odds + both(1.0f);
-    return {reciprocal(d.x), reciprocal(d.y)};
-}
-__device__ __forceinline__ float sigmoid_gate(float z) { return reciprocal(1.0f + exp2_fast(z * kMinusLog2E)); }
+
+// The weights of h and x, each to the relative precision of the odds where it is small and to a few
+// 2^-24 where it is not: a = sigmoid(z) = 1 / (1 + exp(-z)), rest = sigmoid(-z) = exp(-z) a. Beyond
+// |z| = 87.3 the one is zero and the other one: a state or a value behind such a gate does not count,
+// up to the largest float (an infinite one gives a NaN there).
+struct Weights {
+    Pair a, rest;
+
+    __device__ __forceinline__ explicit Weights(Pair odds) {
+        const Pair d = odds + both(1.0f), r = {reciprocal(d.x), reciprocal(d.y)};
+        a = r + both(-kTiny);
+        rest = odds * r;
+    }
+    __device__ __forceinline__ Pair blend(Pair h, Pair x) const { return fma(a, h, rest * x); }
+};
 
 // What the sequences ask for beside their rows, by the warps of the grid in turn, all threads of a
 // block together: one without rows hands on what it was given (`from`, or zeros) to `to`; offsets
@@ -251,6 +303,15 @@ template <int N> struct Row {
             } else {
                 out.v[i] = {raw.v[2 * i], raw.v[2 * i + 1]};
             }
+        }
+        return out;
+    }
+
+    __device__ __forceinline__ Row times(const Row& other) const {
+        Row out;
+#pragma unroll
+        for (int i = 0; i < kPairs; ++i) {
+            out.v[i] = {__fmul_rn(v[i].x, other.v[i].x), __fmul_rn(v[i].y, other.v[i].y)};
         }
         return out;
     }
@@ -514,7 +575,9 @@ template <typename T, int N, int Granule, int Arrays, int Rows, int Stages, int 
 // Takes the ring's memory. A thread composes N pieces of a channel, a run of them; the runs
 // before its own give it the rest.
 template <typename T, int N>
-__device__ __forceinline__ void share_maps(const ScanArgs<T>& p, bool cut, const Row<N>& product, const Row<N>& sum) {
+__device__ __forceinline__ void share_maps(
+    const ScanArgs<T>& p, bool cut, const Row<N>& keep, const Row<N>& rest, const Row<N>& sum
+) {
     static_assert(N % kPieces == 0, "a run holds whole tiles");
     extern __shared__ __align__(16) unsigned char ring[];
     float2* maps = reinterpret_cast<float2*>(ring);   // [pieces of the group][N * lanes]
@@ -524,37 +587,38 @@ __device__ __forceinline__ void share_maps(const ScanArgs<T>& p, bool cut, const
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        maps[N * thread + i] = make_float2(cut ? kReset : product.get(i), sum.get(i));
+        maps[N * thread + i] = make_map(keep.get(i), rest.get(i), sum.get(i), cut);
     }
     __syncthreads();
-    float2 before[N / kPieces], all = make_float2(1.0f, 0.0f);   // each tile of the run
+    Chain before[N / kPieces];   // each tile of the run
+    Chain all;
 #pragma unroll
     for (int k = 0; k < N; ++k) {
         if (k % kPieces == 0) {
             before[k / kPieces] = all;
         }
-        all = compose(all, maps[(run * N + k) * width + lane]);
+        all.add(maps[(run * N + k) * width + lane]);
     }
-    runs[thread] = all;
+    runs[thread] = all.map();
     __syncthreads();
     const int group = blockIdx.x / p.slabs;
     const int channel = (blockIdx.x - group * p.slabs) * width + lane;
     if (channel >= p.channels) {
         return;
     }
-    float2 rest = make_float2(1.0f, 0.0f);
+    Chain earlier;
     for (int k = 0; k < run; ++k) {
-        rest = compose(rest, runs[k * width + lane]);
+        earlier.add(runs[k * width + lane]);
     }
     const int place = group * p.per_group + run * (N / kPieces);
 #pragma unroll
     for (int t = 0; t < N / kPieces; ++t) {
         if (place + t < p.tiles) {
-            p.maps[static_cast<size_t>(place + t) * p.channels + channel] = compose(rest, before[t]);
+            p.maps[static_cast<size_t>(place + t) * p.channels + channel] = earlier.then(before[t]);
         }
     }
     if (run == kMapThreads / width - 1) {
-        p.groups[static_cast<size_t>(group) * p.channels + channel] = compose(rest, all);
+        p.groups[static_cast<size_t>(group) * p.channels + channel] = earlier.then(all);
     }
 }
 
@@ -566,33 +630,17 @@ template <bool Value> struct Flag {
 // rows all take it, instead of both paths one after the other.
 __device__ __forceinline__ bool all_here(bool value) { return __all_sync(__activemask(), value); }
 
-// One row of the recurrence, as h = x + a (h - x): the weights of h and x add up to one whatever
-// the rounding of a, so a long memory does not gather it.
-template <int N> __device__ __forceinline__ void advance(Row<N>& h, const Row<N>& a, const Row<N>& x) {
-#pragma unroll
-    for (int i = 0; i < Row<N>::kPairs; ++i) {
-        h.v[i] = fma(a.v[i], minus(h.v[i], x.v[i]), x.v[i]);
-    }
-}
-
-template <int N> __device__ __forceinline__ Row<N> gates(const Row<N>& z) {
-    Row<N> a;
-#pragma unroll
-    for (int i = 0; i < Row<N>::kPairs; ++i) {
-        a.v[i] = sigmoid_from(exp_minus(z.v[i]));
-    }
-    return a;
-}
-
 // A group's rows are fetched at once and lie together, so this kernel streams: a thread walks
-// eight of them. 960,000 x 64 float16: 48 us, 5.1 of the 6.55 TB/s that a copy moves; the two special
-// functions of a gate alone take 27 us. 200,000 x 96 float32 in 5003 sequences: 45 us, 3.4 TB/s,
-// bound by the searches for a piece's sequence and the rows that start or end one.
+// eight of them. 960,000 x 64 float16: 52 us, 4.7 of the 6.55 TB/s that a copy moves, bound by its
+// instructions; the two special functions of a gate alone take 27 us. 200,000 x 96 float32 in 5003
+// sequences: 46 us, 3.3 TB/s, bound by the searches for a piece's sequence and the rows that start or end one.
 //
-// Backwards, e_t = a_t dh_t is what a row hands to the row before it: e_t = a_t e_{t+1} + a_t dy_t,
-// a chain of the same kind with dy in the place of x. A piece's map needs no walk backwards: what
-// it hands out is the sum of its dy_t times the product of its gates up to t, as far as the first
-// sequence's end.
+// Backwards, e_t = a_t dh_t is what a row hands to the row before it: e_t = a_t (e_{t+1} + dy_t), a
+// chain of the same kind, from the piece's last row to its first, or from the last row of the first
+// sequence in it.
+//
+// Here and in the gradient kernel dh_t = a_{t+1} dh_{t+1} + dy_t is one multiply-add. A product of pairs
+// and a sum behind it become one or not as the compiler likes, and results would depend on the launch.
 template <typename T, int Granule, bool Backward>
 __global__ void __launch_bounds__(kMapThreads, 6) recurrence_maps_kernel(ScanArgs<T> p) {
     constexpr int N = kMapBytes / static_cast<int>(sizeof(T)), R = kPieceRows;
@@ -607,7 +655,8 @@ __global__ void __launch_bounds__(kMapThreads, 6) recurrence_maps_kernel(ScanArg
             p.arrived[i] = 0;
         }
     }
-    Row<N> prod = Row<N>::filled(1.0f), sum = Row<N>::filled(0.0f);
+    Row<N> keep = Row<N>::filled(1.0f), rest = Row<N>::filled(0.0f), sum = rest;   // A, 1 - A and H
+    Row<N> share = keep;   // backwards: sum is dh of a row, and share of it reaches the next one
     bool cut = false;
     const int first = piece * R, rows = p.order.rows - first;
     if (piece >= 0 && rows > 0 && lanes.count > 0) {
@@ -622,49 +671,42 @@ __global__ void __launch_bounds__(kMapThreads, 6) recurrence_maps_kernel(ScanArg
         ring.drain();
         const auto scan = [&](auto marked) {
             constexpr bool kMarked = decltype(marked)::value;
+            const int live = Backward && kMarked ? cursor.end - first : R;   // rows that hand something out
+            if (Backward && kMarked && (cursor.begin > first || live <= R)) {
+                cut = true;
+            }
 #pragma unroll
-            for (int r = 0; r < R; ++r) {
-                if (kMarked && first + r < cursor.begin) {
-                    cut = true;
-                    if constexpr (Backward) {
-                        break;   // a row outside all sequences hands nothing out
-                    } else {
-                        sum = Row<N>::filled(0.0f);
-                        continue;
-                    }
+            for (int i = 0; i < R; ++i) {
+                const int r = Backward ? R - 1 - i : i;
+                if (kMarked && (Backward ? cursor.begin > first || r >= live : first + r < cursor.begin)) {
+                    cut = true;   // outside all sequences, or behind the first one's end
+                    sum = Row<N>::filled(0.0f);   // backwards no row with anything comes before
+                    continue;
                 }
-                const Row<N> a = gates(ring.row(0, 1, r, lanes.odd(p.z, p.z_stride, p.order, first + r)));
-                Row<N> value = ring.row(0, 0, r, Backward ? lanes.odd(p.dy, p.dy_stride, p.order, first + r)
-                                                          : lanes.odd(p.x, p.x_stride, p.order, first + r));
-                const bool ends = kMarked && first + r == cursor.end - 1;
-                if (Backward && ends) {
-                    const Row<N> more = lanes.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
-#pragma unroll
-                    for (int i = 0; i < Row<N>::kPairs; ++i) {
-                        value.v[i] = value.v[i] + more.v[i];
-                    }
+                const Row<N> z = ring.row(0, 1, r, lanes.odd(p.z, p.z_stride, p.order, first + r));
+                const Row<N> value = ring.row(0, 0, r, Backward ? lanes.odd(p.dy, p.dy_stride, p.order, first + r)
+                                                                : lanes.odd(p.x, p.x_stride, p.order, first + r));
+                if (Backward && kMarked && r == live - 1) {
+                    sum = lanes.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
                 }
                 if (!Backward && kMarked && first + r == cursor.begin) {
                     cut = true;
                     sum = lanes.state(p.initial, p.order.sequence(cursor.j), p.channels);
                 }
 #pragma unroll
-                for (int i = 0; i < Row<N>::kPairs; ++i) {
-                    prod.v[i] = prod.v[i] * a.v[i];
+                for (int c = 0; c < Row<N>::kPairs; ++c) {
+                    const Weights w(odds_of(z.v[c]));
+                    rest.v[c] = fma(keep.v[c], w.rest, rest.v[c]);
+                    keep.v[c] = keep.v[c] * w.a;
                     if constexpr (Backward) {
-                        sum.v[i] = fma(prod.v[i], value.v[i], sum.v[i]);
-                    }
-                }
-                if constexpr (!Backward) {
-                    advance(sum, a, value);
-                }
-                if (ends) {
-                    if constexpr (Backward) {
-                        cut = true;
-                        break;
+                        sum.v[c] = fma(share.v[c], sum.v[c], value.v[c]);
+                        share.v[c] = w.a;
                     } else {
-                        cursor.next(p.order);
+                        sum.v[c] = w.blend(sum.v[c], value.v[c]);
                     }
+                }
+                if (!Backward && kMarked && first + r == cursor.end - 1) {
+                    cursor.next(p.order);
                 }
             }
         };
@@ -674,11 +716,14 @@ __global__ void __launch_bounds__(kMapThreads, 6) recurrence_maps_kernel(ScanArg
             scan(Flag<true>{});
         }
     }
-    share_maps(p, cut, prod, sum);
+    if constexpr (Backward) {
+        sum = sum.times(share);
+    }
+    share_maps(p, cut, keep, rest, sum);
 }
 
-// 960,000 x 64 float16 with carries: 63 us, 6.3 TB/s, the memory's rate; 200,000 x 96 float32 in 5003
-// sequences: 42 us, 5.7 TB/s.
+// 960,000 x 64 float16 with carries: 60 us, 6.6 TB/s, the memory's rate; 200,000 x 96 float32 in 5003
+// sequences: 43 us, 5.7 TB/s.
 constexpr int kRingRows = 2, kRingStages = 4;
 
 template <typename T, int Granule>
@@ -729,8 +774,12 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<
                 if (decltype(marked)::value && row + r == cursor.begin) {
                     h = lanes.state(p.initial, p.order.sequence(cursor.j), p.channels);
                 }
-                advance(h, gates(ring.row(stage, 1, r, lanes.odd(p.z, p.z_stride, p.order, row + r))),
-                        ring.row(stage, 0, r, lanes.odd(p.x, p.x_stride, p.order, row + r)));
+                const Row<N> z = ring.row(stage, 1, r, lanes.odd(p.z, p.z_stride, p.order, row + r));
+                const Row<N> x = ring.row(stage, 0, r, lanes.odd(p.x, p.x_stride, p.order, row + r));
+#pragma unroll
+                for (int i = 0; i < Row<N>::kPairs; ++i) {
+                    h.v[i] = Weights(odds_of(z.v[i])).blend(h.v[i], x.v[i]);
+                }
                 if (decltype(marked)::value && row + r < cursor.begin) {
                     h = Row<N>::filled(0.0f);
                 }
@@ -751,9 +800,9 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<
     }
 }
 
-// Batches of rows from the last to the first. With q_t = a_t (h_{t-1} - x_t): h_t = x_t + q_t,
-// and dz_t = dx_t q_t. 960,000 x 64 float16: 102 us, 6.3 TB/s, the memory's rate; 200,000 x 96 float32
-// in 5003 sequences: 85 us, 4.6 TB/s.
+// Batches of rows from the last to the first: h again up to the batch's end, with
+// q_t = a_t (h_{t-1} - x_t), then dh_t back from there, and dz_t = dx_t q_t. 960,000 x 64 float16:
+// 102 us, 6.3 TB/s, the memory's rate; 200,000 x 96 float32 in 5003 sequences: 88 us, 4.5 TB/s.
 template <typename T, int Granule>
 __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanArgs<T> p) {
     constexpr int N = kGradientBytes / static_cast<int>(sizeof(T)), R = kCarryRows, P = Row<N>::kPairs;
@@ -826,39 +875,45 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
                 const Row<N> xr = ring.row(stage, 0, r, lanes.odd(p.x, p.x_stride, p.order, row + r));
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
-                    odds[r].v[i] = exp_minus({max_or_nan(zr.v[i].x, kLowestGate), max_or_nan(zr.v[i].y, kLowestGate)});
-                    q[r].v[i] = sigmoid_from(odds[r].v[i]) * minus(h.v[i], xr.v[i]);
-                    h.v[i] = xr.v[i] + q[r].v[i];
+                    odds[r].v[i] = odds_of(zr.v[i]);
+                    const Weights w(odds[r].v[i]);
+                    q[r].v[i] = w.a * minus(h.v[i], xr.v[i]);
+                    h.v[i] = w.blend(h.v[i], xr.v[i]);
                 }
                 if (decltype(marked)::value && (tails >> r & 1u)) {
                     cursor.next(p.order);
                 }
             }
+            Row<N> dh = e, share = Row<N>::filled(1.0f);   // share of dh reaches the row before
 #pragma unroll
             for (int r = R - 1; r >= 0; --r) {
                 if (decltype(marked)::value && (tails >> r & 1u)) {
                     cursor.back(p.order);
-                    e = lanes.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
+                    dh = lanes.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
+                    share = Row<N>::filled(1.0f);
                 }
                 const Row<N> up = ring.row(stage, 2, r, lanes.odd(p.dy, p.dy_stride, p.order, row + r));
                 Row<N> dx, dz;
 #pragma unroll
                 for (int i = 0; i < P; ++i) {
-                    e.v[i] = sigmoid_from(odds[r].v[i]) * (up.v[i] + e.v[i]);
-                    dx.v[i] = odds[r].v[i] * e.v[i];   // exp(-z) sigmoid(z) dh = sigmoid(-z) dh
+                    const Weights w(odds[r].v[i]);
+                    dh.v[i] = fma(share.v[i], dh.v[i], up.v[i]);
+                    share.v[i] = w.a;
+                    dx.v[i] = w.rest * dh.v[i];
                     dz.v[i] = dx.v[i] * q[r].v[i];
                 }
                 if (decltype(marked)::value && (dead >> r & 1u)) {
-                    dx = dz = e = Row<N>::filled(0.0f);
+                    dx = dz = dh = share = Row<N>::filled(0.0f);
                 }
                 if (!decltype(marked)::value || row + r < end) {
                     lanes.store(p.dx + at0 + r * down, dx);
                     lanes.store(p.dz + at0 + r * down, dz);
                 }
                 if (decltype(marked)::value && (heads >> r & 1u)) {
-                    lanes.store_state(p.dinitial, p.order.sequence(cursor.j), p.channels, e);
+                    lanes.store_state(p.dinitial, p.order.sequence(cursor.j), p.channels, dh.times(share));
                 }
             }
+            e = dh.times(share);
         };
         if (covered) {
             differentiate(Flag<false>{});
@@ -869,63 +924,57 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
     }
 }
 
-// A run of kRun maps of a channel by every warp of a block, kWindow by the block: each becomes
-// the map of those before it, and the map of all comes back to every thread.
+// A run of kRun maps of a channel by every warp of a block, kWindow by the block.
 constexpr int kScanWarps = 8, kRun = kWindow / kScanWarps;
 
-__device__ __forceinline__ float2 scan_maps(float2 (&maps)[kRun], float2 (&shared)[kScanWarps][32]) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float2 all = make_float2(1.0f, 0.0f);
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-        const float2 own = maps[i];
-        maps[i] = all;
-        all = compose(all, own);
-    }
-    __syncthreads();   // a second call writes what the first one read
-    shared[warp][lane] = all;
-    __syncthreads();
-    float2 before = make_float2(1.0f, 0.0f), total = before;
-#pragma unroll
-    for (int w = 0; w < kScanWarps; ++w) {
-        before = w == warp ? total : before;
-        total = compose(total, shared[w][lane]);
-    }
-#pragma unroll
-    for (int i = 0; i < kRun; ++i) {
-        maps[i] = compose(before, maps[i]);
-    }
-    return total;
-}
-
-// Block: a window of groups for 32 channels (7500 groups of 64 channels: 8 us, a chain of latencies). The last block of these channels to be done goes on
-// to the states of the windows: which block that is does not change what it computes.
+// Block: a window of groups for 32 channels. The last block of these channels to be done goes on to
+// the states of the windows: which block that is does not change what it computes. 7500 groups of
+// 64 channels: 8.4 us, a chain of latencies, among them those of its instructions, which every
+// launch fetches anew: with all loops unrolled it takes 10.6 us.
 __global__ void __launch_bounds__(32 * kScanWarps) recurrence_scan_kernel(
     float2* groups, int count, int channels, float2* windows, float* states, int* arrived
 ) {
-    __shared__ float2 shared[kScanWarps][32];
+    __shared__ float2 held[kWindow][32];       // the maps: a thread reads what it wrote itself
+    __shared__ float2 shared[kScanWarps][32];   // of the runs
     __shared__ bool last;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = blockIdx.y * 32 + lane;
-    const auto load = [&](const float2* from, int first, int end, float2 (&maps)[kRun]) {
+    // maps `first` to `first` + kRun - 1, and the map of all of them in `shared`
+    const auto load = [&](const float2* from, int first, int end) {
+        float2 maps[kRun];
 #pragma unroll
         for (int i = 0; i < kRun; ++i) {
             maps[i] = c < channels && first + i < end ? __ldcg(from + static_cast<size_t>(first + i) * channels + c)
-                                                      : make_float2(1.0f, 0.0f);
+                                                      : identity();
         }
-    };
-    float2 maps[kRun];
-    int first = blockIdx.x * kWindow + warp * kRun;
-    load(groups, first, count, maps);
-    const float2 total = scan_maps(maps, shared);
 #pragma unroll
+        for (int i = 0; i < kRun; ++i) {
+            held[warp * kRun + i][lane] = maps[i];
+        }
+        Chain run;
+#pragma unroll 1
+        for (int i = 0; i < kRun; ++i) {
+            run.add(held[warp * kRun + i][lane]);
+        }
+        shared[warp][lane] = run.map();
+        __syncthreads();
+    };
+    int first = blockIdx.x * kWindow + warp * kRun;
+    load(groups, first, count);
+    Chain before;
+#pragma unroll 1
+    for (int w = 0; w < warp; ++w) {
+        before.add(shared[w][lane]);
+    }
+#pragma unroll 1
     for (int i = 0; i < kRun; ++i) {
         if (c < channels && first + i < count) {
-            groups[static_cast<size_t>(first + i) * channels + c] = maps[i];
+            groups[static_cast<size_t>(first + i) * channels + c] = before.map();
         }
+        before.add(held[warp * kRun + i][lane]);
     }
-    if (warp == 0 && c < channels) {
-        __stcg(windows + static_cast<size_t>(blockIdx.x) * channels + c, total);
+    if (warp == kScanWarps - 1 && c < channels) {
+        __stcg(windows + static_cast<size_t>(blockIdx.x) * channels + c, before.map());
     }
     __threadfence();
     __syncthreads();
@@ -941,15 +990,21 @@ __global__ void __launch_bounds__(32 * kScanWarps) recurrence_scan_kernel(
     float h = 0.0f;
     for (int base = 0; base < windows_count; base += kWindow) {
         first = base + warp * kRun;
-        load(windows, first, windows_count, maps);
-        const float2 all = scan_maps(maps, shared);
-#pragma unroll
+        load(windows, first, windows_count);
+        float reached = h;   // the state before the warp's run, h the one behind all
+#pragma unroll 1
+        for (int w = 0; w < kScanWarps; ++w) {
+            reached = w == warp ? h : reached;
+            h = apply(shared[w][lane], h);
+        }
+#pragma unroll 1
         for (int i = 0; i < kRun; ++i) {
             if (c < channels && first + i < windows_count) {
-                states[static_cast<size_t>(first + i) * channels + c] = apply(maps[i], h);
+                states[static_cast<size_t>(first + i) * channels + c] = reached;
             }
+            reached = apply(held[warp * kRun + i][lane], reached);
         }
-        h = apply(all, h);
+        __syncthreads();   // the next turn writes what this one reads
     }
 }
 
@@ -973,8 +1028,7 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(
     Pack<float, V> now;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const float a = sigmoid_gate(zs.get(i));
-        now.v[i] = fmaf(a, old.v[i] - xs.get(i), xs.get(i));
+        now.v[i] = Weights(odds_of(both(zs.get(i)))).blend(both(old.v[i]), both(xs.get(i))).x;
         y.set(i, now.v[i]);
     }
     store_pack<T, V>(h + row * channels + c, y);
