@@ -511,7 +511,8 @@ int lat_dropout(
  * is dense; final_state [sequences, channels] float32 (or NULL) is the h after the last row (an
  * empty sequence hands its initial state on). carries (NULL unless a backward pass follows):
  * float32 [lat_recurrence_carry_rows(rows), channels], the h before every eighth row. Bitwise
- * repeatable. At most 2097120 channels. */
+ * repeatable. At most 2097120 channels, 2147482623 rows and 2147483583 sequences. Weights a or
+ * 1 - a below 2^-126 count as zero. */
 size_t lat_recurrence_workspace_bytes(int32_t dtype, int32_t rows, int32_t channels);
 int32_t lat_recurrence_carry_rows(int32_t rows);
 int lat_recurrence_forward(

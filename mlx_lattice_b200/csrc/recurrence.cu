@@ -1037,7 +1037,10 @@ __global__ void __launch_bounds__(256) recurrence_step_kernel(
 
 // ---- host -------------------------------------------------------------------------
 
-constexpr int kMaxRows = 0x7fffffff - kTileRows;   // row numbers of the last tile stay in an int
+// Row numbers of the last group, places behind the last sequence that a search tries and their sums
+// stay in an int.
+constexpr int kMaxRows = 0x7fffffff - kMapThreads * kPieceRows;
+constexpr int kMaxSequences = 0x7fffffff - 64;
 
 constexpr int kMaxChannels = 65535 * kScanChannels;   // of the scan kernel's grid
 
@@ -1261,6 +1264,7 @@ int lat_recurrence_forward(
     LAT_REQUIRE(channels <= kMaxChannels, "the recurrence supports at most 2097120 channels.");
     LAT_REQUIRE(sequences >= 0 && (sequences == 0 || offsets != nullptr),
                 "offsets must hold one int32 entry per sequence and one more.");
+    LAT_REQUIRE(sequences <= kMaxSequences, "the recurrence supports at most 2147483583 sequences.");
     cudaStream_t stream = as_stream(stream_ptr);
     if (rows == 0) {
         return hand_over(initial_state, final_state, sequences, channels, stream);
@@ -1289,6 +1293,7 @@ int lat_recurrence_backward(
     LAT_REQUIRE(channels <= kMaxChannels, "the recurrence supports at most 2097120 channels.");
     LAT_REQUIRE(sequences >= 0 && (sequences == 0 || offsets != nullptr),
                 "offsets must hold one int32 entry per sequence and one more.");
+    LAT_REQUIRE(sequences <= kMaxSequences, "the recurrence supports at most 2147483583 sequences.");
     cudaStream_t stream = as_stream(stream_ptr);
     if (rows == 0) {
         return hand_over(grad_final, grad_initial, sequences, channels, stream);

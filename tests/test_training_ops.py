@@ -110,3 +110,27 @@ def test_module_arguments():
         nn.Dropout(1.0)
     assert nn.GatedRecurrence(reverse=True).reverse
     assert {'gated_recurrence', 'gated_recurrence_step', 'sequence_offsets'} <= set(ops.__all__)
+
+
+def test_recurrence_sizes_near_the_end_of_an_int_are_refused():
+    """Row numbers of the last group (1024 rows), and places that a search tries behind the last
+    sequence, have to stay within 32 bits; calls beyond end before anything runs."""
+    lib = _native.load()
+    buf = ctypes.c_void_p(4096)
+    top = 2 ** 31 - 1
+
+    def forward(rows, sequences):
+        return lib.lat_recurrence_forward(F16, buf, 1, buf, 1, rows, 1, buf, sequences, None, 0, buf, None, None, None,
+                                          0, None, None)
+
+    def backward(rows, sequences):
+        return lib.lat_recurrence_backward(F16, buf, 1, None, buf, 1, buf, 1, rows, 1, buf, sequences, None, 0, buf, buf,
+                                           buf, None, None, 0, None, None)
+
+    for call in (forward, backward):
+        for rows in (top - 32, top - 63, top - 1023):
+            _refused(call(rows, 1), 'shape (N, C)')
+        for sequences in (top, top - 1, top - 16):
+            _refused(call(64, sequences), 'sequences')
+        # the largest ones only lack a workspace
+        assert call(top - 1024, top - 64) == _native.LAT_WORKSPACE_TOO_SMALL
