@@ -195,14 +195,29 @@ __device__ __forceinline__ void visit_sequences(
 struct Cursor {
     int j, begin, end;
 
+    // Sequences without rows are stepped over one at a time at first, then by bisection of the offsets:
+    // a run of a million of them costs twenty dependent loads, not a million.
+    static constexpr int kSteps = 4;
+
     __device__ __forceinline__ void settle(const Order& order) {
-        while (j < order.sequences) {
+        for (int step = 0; j < order.sequences; ++step) {
             begin = order.begin(j);
             end = order.begin(j + 1);
             if (end > begin) {
                 return;
             }
-            ++j;   // no rows
+            ++j;
+            if (step >= kSteps) {   // on to the first sequence that ends behind this place
+                int high = order.sequences;
+                while (j < high) {
+                    const int middle = j + (high - j) / 2;
+                    if (order.begin(middle + 1) > begin) {
+                        high = middle;
+                    } else {
+                        j = middle + 1;
+                    }
+                }
+            }
         }
         begin = end = 0x7fffffff;
     }
@@ -230,13 +245,26 @@ struct Cursor {
 
     // the sequence before, where there is one
     __device__ __forceinline__ bool back(const Order& order) {
-        for (int k = j - 1; k >= 0; --k) {
+        int k = j - 1;
+        for (int step = 0; k >= 0; ++step) {
             const int b = order.begin(k), e = order.begin(k + 1);
             if (e > b) {
                 j = k;
                 begin = b;
                 end = e;
                 return true;
+            }
+            --k;
+            if (step >= kSteps) {   // back to the last sequence that begins before this place
+                int low = -1;
+                while (low < k) {
+                    const int middle = k - (k - low) / 2;
+                    if (order.begin(middle) < b) {
+                        low = middle;
+                    } else {
+                        k = middle - 1;
+                    }
+                }
             }
         }
         return false;
@@ -802,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 3) recurrence_apply_kernel(ScanArgs<
 
 // Batches of rows from the last to the first: h again up to the batch's end, with
 // q_t = a_t (h_{t-1} - x_t), then dh_t back from there, and dz_t = dx_t q_t. 960,000 x 64 float16:
-// 102 us, 6.3 TB/s, the memory's rate; 200,000 x 96 float32 in 5003 sequences: 88 us, 4.5 TB/s.
+// 101 us, 6.3 TB/s, the memory's rate; 200,000 x 96 float32 in 5003 sequences: 84 us, 4.7 TB/s.
 template <typename T, int Granule>
 __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanArgs<T> p) {
     constexpr int N = kGradientBytes / static_cast<int>(sizeof(T)), R = kCarryRows, P = Row<N>::kPairs;
@@ -811,6 +839,10 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
     const int span = static_cast<int>(blockIdx.x) / p.slabs * per_block + static_cast<int>(threadIdx.x) / p.lanes;
     const Channels<T, N, Granule> lanes(p, blockIdx.x % p.slabs);
     const Ring<T, N, Granule, 3, R, 2> ring;
+    // Of each row of a batch that starts or ends a sequence. In local memory, as the loop that writes it is
+    // not unrolled: there are no registers left, and shared memory would be the first-level cache's, which
+    // the copies come through (102 us become 130).
+    int owner[R];
     visit_sequences(p.order, p.dfinal, p.dinitial, p.channels, nullptr);
     if (span >= spans || lanes.count == 0) {
         return;
@@ -848,13 +880,17 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
             cursor = before;
         }
         const bool covered = all_here(cursor.covers(row, R));
-        // of the batch's rows: start a sequence, end one, lie outside all
+        // of the batch's rows: start a sequence, end one (whose numbers are kept), lie outside all
         unsigned heads = 0, tails = 0, dead = 0;
         if (!covered) {
             Cursor at = cursor;
+#pragma unroll 1
             for (int r = 0; r < R; ++r) {
                 dead |= row + r < at.begin ? 1u << r : 0u;
                 heads |= row + r == at.begin ? 1u << r : 0u;
+                if (row + r == at.begin || row + r == at.end - 1) {
+                    owner[r] = p.order.sequence(at.j);
+                }
                 if (row + r == at.end - 1) {
                     tails |= 1u << r;
                     at.next(p.order);
@@ -869,7 +905,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
 #pragma unroll
             for (int r = 0; r < R; ++r) {
                 if (decltype(marked)::value && (heads >> r & 1u)) {
-                    h = lanes.state(p.initial, p.order.sequence(cursor.j), p.channels);
+                    h = lanes.state(p.initial, owner[r], p.channels);
                 }
                 const Row<N> zr = ring.row(stage, 1, r, lanes.odd(p.z, p.z_stride, p.order, row + r));
                 const Row<N> xr = ring.row(stage, 0, r, lanes.odd(p.x, p.x_stride, p.order, row + r));
@@ -880,16 +916,12 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
                     q[r].v[i] = w.a * minus(h.v[i], xr.v[i]);
                     h.v[i] = w.blend(h.v[i], xr.v[i]);
                 }
-                if (decltype(marked)::value && (tails >> r & 1u)) {
-                    cursor.next(p.order);
-                }
             }
             Row<N> dh = e, share = Row<N>::filled(1.0f);   // share of dh reaches the row before
 #pragma unroll
             for (int r = R - 1; r >= 0; --r) {
                 if (decltype(marked)::value && (tails >> r & 1u)) {
-                    cursor.back(p.order);
-                    dh = lanes.state(p.dfinal, p.order.sequence(cursor.j), p.channels);
+                    dh = lanes.state(p.dfinal, owner[r], p.channels);
                     share = Row<N>::filled(1.0f);
                 }
                 const Row<N> up = ring.row(stage, 2, r, lanes.odd(p.dy, p.dy_stride, p.order, row + r));
@@ -910,7 +942,7 @@ __global__ void __launch_bounds__(kThreads, 2) recurrence_gradient_kernel(ScanAr
                     lanes.store(p.dz + at0 + r * down, dz);
                 }
                 if (decltype(marked)::value && (heads >> r & 1u)) {
-                    lanes.store_state(p.dinitial, p.order.sequence(cursor.j), p.channels, dh.times(share));
+                    lanes.store_state(p.dinitial, owner[r], p.channels, dh.times(share));
                 }
             }
             e = dh.times(share);
@@ -1138,7 +1170,8 @@ int launch_scan(ScanArgs<T> p, void* workspace, size_t bytes, cudaStream_t strea
         // leave multiprocessors idle (2168 x 13 float16 in 94 sequences: 43 us, with two tiles 77;
         // 15,191 x 12 float32 in 134: 16 against 24).
         p.span_tiles = blocks_of(2) >= 2 * 148 ? 2 : 1;
-        return launch_walk(recurrence_gradient_kernel<T, Granule>, kThreads, Ring<T, M, Granule, 3, kCarryRows, 2>::kBytes,
+        constexpr int kGradientRing = Ring<T, M, Granule, 3, kCarryRows, 2>::kBytes;
+        return launch_walk(recurrence_gradient_kernel<T, Granule>, kThreads, kGradientRing,
                            blocks_of(p.span_tiles), p, stream);
     } else {
         const int per_block = kThreads / p.lanes;

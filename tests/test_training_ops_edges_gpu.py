@@ -293,3 +293,70 @@ def test_recurrence_of_values_near_the_largest(cuda):
     want = _reference(x, z, [0, 200], state, False, zeros, zeros[:1])
     _within(h, *want['h'], torch.float32, 'h')
     _within(final, *want['final'], torch.float32, 'final')
+
+
+# --------------------------------------------------------------------------- #
+# long runs of empty sequences
+# --------------------------------------------------------------------------- #
+
+
+@pytest.mark.parametrize('reverse', [False, True])
+def test_a_million_empty_sequences_between_two(cuda, reverse):
+    """A pool of streams that is mostly unused: values as without the empty ones, and the time of a
+    few searches, not of a walk over a million entries (tens of milliseconds in each kernel)."""
+    from mlx_lattice_b200 import _ext
+
+    rng = np.random.default_rng(31)
+    rows, empty = 6000, 1_000_000
+    x, z, dy = (_randn(rng, rows, 8) for _ in range(3))
+    few = torch.tensor([0, 2990, 3001, rows], dtype=torch.int32, device=cuda)
+    many = torch.cat([few[:1], torch.full((empty,), 2990, dtype=torch.int32, device=cuda),
+                      torch.full((empty,), 3001, dtype=torch.int32, device=cuda), few[3:]])
+    h, _, carries = _ext.recurrence_forward(x, z, few, None, reverse, want_carries=True)
+    dx, dz, _ = _ext.recurrence_backward(dy, None, x, z, few, None, reverse, carries)
+
+    def run():
+        got, _, kept = _ext.recurrence_forward(x, z, many, None, reverse, want_carries=True)
+        return (got, *_ext.recurrence_backward(dy, None, x, z, many, None, reverse, kept)[:2])
+
+    assert all(torch.equal(a, b) for a, b in zip(run(), (h, dx, dz)))
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    begin.record()
+    run()
+    end.record()
+    end.synchronize()
+    assert begin.elapsed_time(end) < 20.0, begin.elapsed_time(end)
+    _ext.check_status(cuda)
+
+
+@pytest.mark.parametrize('reverse', [False, True])
+def test_falling_offsets_stay_within_the_arrays(cuda, reverse):
+    """Offsets that fall, with runs of empty sequences longer than those stepped over one by one:
+    both passes report them, and write nothing around their outputs."""
+    from mlx_lattice_b200 import _ext, _native
+
+    lib, pad, rows = _native.load(), 64, 200
+    rng = np.random.default_rng(33)
+    x = _randn(rng, rows, 4)
+    for trial in range(8):
+        cuts = rng.integers(-20, rows + 20, size=40)
+        cuts[5:20] = cuts[4]
+        off = torch.from_numpy(cuts.astype(np.int32)).to(cuda)
+        buffers = [torch.full((n * 4 + 2 * pad,), 7.0, device=cuda) for n in (rows, 39, rows, rows, 39)]
+        h, final, dx, dz, dinitial = (b[pad:].data_ptr() for b in buffers)
+        state = _randn(rng, 39, 4)
+        carries = torch.zeros((lib.lat_recurrence_carry_rows(rows), 4), device=cuda)
+        need = lib.lat_recurrence_workspace_bytes(0, rows, 4)
+        workspace = torch.empty(need, dtype=torch.uint8, device=cuda)
+        status, stream = torch.zeros(1, dtype=torch.int32, device=cuda), torch.cuda.current_stream().cuda_stream
+        assert lib.lat_recurrence_forward(
+            0, x.data_ptr(), 4, x.data_ptr(), 4, rows, 4, off.data_ptr(), 39, state.data_ptr(), int(reverse), h, final,
+            carries.data_ptr(), workspace.data_ptr(), need, status.data_ptr(), stream) == _native.LAT_OK
+        assert lib.lat_recurrence_backward(
+            0, x.data_ptr(), 4, state.data_ptr(), x.data_ptr(), 4, x.data_ptr(), 4, rows, 4, off.data_ptr(), 39,
+            state.data_ptr(), int(reverse), carries.data_ptr(), dx, dz, dinitial, workspace.data_ptr(), need,
+            status.data_ptr(), stream) == _native.LAT_OK
+        assert int(status) != 0
+        for buffer in buffers:
+            assert (buffer[:pad] == 7).all() and (buffer[-pad:] == 7).all()
+    _ext.check_status(cuda)
