@@ -329,6 +329,34 @@ def test_a_million_empty_sequences_between_two(cuda, reverse):
     _ext.check_status(cuda)
 
 
+@pytest.mark.parametrize('rows', [64, 6000])
+def test_a_million_empty_sequences_hand_on_their_states(cuda, rows):
+    """Few rows, many states: all blocks that there are copy them (one block alone takes 60 ms)."""
+    from mlx_lattice_b200 import _ext
+
+    rng = np.random.default_rng(37)
+    many = 1_000_000
+    x, dy = _randn(rng, rows, 16), _randn(rng, rows, 16)
+    offsets = torch.full((many + 1,), rows // 2, dtype=torch.int32, device=cuda)
+    offsets[0], offsets[-1] = 0, rows
+    state = torch.randn((many, 16), device=cuda)
+    flow = torch.randn((many, 16), device=cuda)
+
+    def run():
+        h, final, carries = _ext.recurrence_forward(x, x, offsets, state, want_state=True, want_carries=True)
+        return final, _ext.recurrence_backward(dy, flow, x, x, offsets, state, False, carries, want_initial=True)[2]
+
+    final, dstate = run()
+    assert torch.equal(final[1:-1], state[1:-1]) and torch.equal(dstate[1:-1], flow[1:-1])
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    begin.record()
+    run()
+    end.record()
+    end.synchronize()
+    assert begin.elapsed_time(end) < 20.0, begin.elapsed_time(end)
+    _ext.check_status(cuda)
+
+
 @pytest.mark.parametrize('reverse', [False, True])
 def test_falling_offsets_stay_within_the_arrays(cuda, reverse):
     """Offsets that fall, with runs of empty sequences longer than those stepped over one by one:
