@@ -417,6 +417,10 @@ std::tuple<Tensor, Tensor> recurrence_step(
     const Tensor state = state_argument(*state_in, "state", feats.rows, feats);
     Tensor next = out_state_in.value_or(Tensor());
     if (next.defined()) {
+        // a state that this function returned may go on; another one would keep a graph that its new
+        // values do not come from
+        REQUIRE(!wants_gradient({next}) || dynamic_cast<torch::autograd::Error*>(next.grad_fn().get()) != nullptr,
+                "out_state must not require a gradient.");
         REQUIRE(state_argument(next, "out_state", feats.rows, feats).is_same(next), "out_state must be contiguous.");
         // a thread reads and writes one place of the state; every other overlap is a race
         REQUIRE(next.const_data_ptr() == state.const_data_ptr() || !overlap(next, state),
@@ -431,6 +435,11 @@ std::tuple<Tensor, Tensor> recurrence_step(
     check(lat_recurrence_step(
         dtype, data(feats.t), feats.stride, data(gate.t), gate.stride, floats(state), feats.rows,
         static_cast<int32_t>(feats.channels), mutable_data(out), mutable_floats(next), stream_of(feats)));
+    if (wants_gradient({feats_in, gate_in, *state_in})) {
+        const variable_list results =
+            raising({out, next}, "gated_recurrence_step has no gradient: use gated_recurrence, or torch.no_grad()");
+        return {results[0], results[1]};
+    }
     return {out, next};
 }
 

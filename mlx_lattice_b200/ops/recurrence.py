@@ -48,7 +48,8 @@ def gated_recurrence_step(
 ) -> tuple[SparseTensor, torch.Tensor]:
     """One new row for each of ``N`` streams: row ``i`` of ``x`` and ``gate`` advances row ``i``
     of the float32 ``state``. Returns the sparse tensor of the new ``h`` and the next state,
-    written to ``out_state`` when given (which may be ``state``). For serving: no gradient."""
+    written to ``out_state`` when given (which may be ``state``). For serving: it has no gradient, and
+    results that depend on something with one raise when they are differentiated."""
     h, state = _ext.recurrence_step(x.feats, _gate(x, gate), state, out_state)
     return x.replace(feats=h), state
 

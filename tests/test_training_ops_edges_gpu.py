@@ -388,3 +388,42 @@ def test_falling_offsets_stay_within_the_arrays(cuda, reverse):
         for buffer in buffers:
             assert (buffer[:pad] == 7).all() and (buffer[-pad:] == 7).all()
     _ext.check_status(cuda)
+
+
+# --------------------------------------------------------------------------- #
+# the step and gradients
+# --------------------------------------------------------------------------- #
+
+
+def test_recurrence_step_does_not_lose_a_gradient_silently(cuda):
+    """The step has values only: results that depend on something with a gradient say so when one
+    is asked of them. Streams may go on from such a state, in place too."""
+    from mlx_lattice_b200 import _ext, ops
+
+    rng = np.random.default_rng(17)
+    feats, gate, state = (_randn(rng, 6, 8) for _ in range(3))
+    want, after = ops.gated_recurrence_step(_sparse(feats), gate, state)
+    assert not want.feats.requires_grad and not after.requires_grad
+    for place in range(3):
+        args = [feats, gate, state]
+        args[place] = args[place].clone().requires_grad_(True)
+        h, new = ops.gated_recurrence_step(_sparse(args[0]), args[1], args[2])
+        assert torch.equal(h.feats, want.feats) and torch.equal(new, after)
+        for result in (h.feats, new):
+            with pytest.raises(RuntimeError, match='gated_recurrence'):
+                result.sum().backward()
+        with torch.no_grad():
+            h, new = ops.gated_recurrence_step(_sparse(args[0]), args[1], args[2])
+        assert not h.feats.requires_grad and not new.requires_grad
+    leaf, held = feats.clone().requires_grad_(True), state.clone()
+    h, new = ops.gated_recurrence_step(_sparse(leaf), gate, held, out_state=held)
+    assert torch.equal(held, after) and new.data_ptr() == held.data_ptr()
+    h, new = ops.gated_recurrence_step(_sparse(leaf), gate, new, out_state=new)
+    with pytest.raises(RuntimeError, match='gated_recurrence'):
+        h.feats.sum().backward()
+    with pytest.raises(ValueError, match='out_state'):
+        ops.gated_recurrence_step(_sparse(feats), gate, state, out_state=state.clone().requires_grad_(True))
+    with torch.no_grad():
+        owner = state.clone().requires_grad_(True)
+        _ext.recurrence_step(feats, gate, state, owner)
+        assert torch.equal(owner, after)
