@@ -1173,7 +1173,8 @@ def row_norm_backward(grad, feats, weight, mean, rstd, rms: bool, want_weight: b
 
 
 def row_norm_recorded(feats, weight, bias, eps: float, rms: bool):
-    """The normalised features recorded for a gradient; None where no argument asks for one."""
+    """The normalised features recorded for the gradient that an argument asks for; None where
+    none does."""
     return bindings().row_norm_recorded(feats, weight, bias, eps, rms)
 
 

@@ -103,10 +103,7 @@ def layer_norm(x: SparseTensor, *, weight=None, bias=None, eps: float = 1e-5) ->
     Differentiable in ``x.feats``, ``weight`` and ``bias``."""
     if eps <= 0:
         raise ValueError('eps must be positive.')
-    feats = _ext.row_norm_recorded(x.feats, weight, bias, eps, rms=False)
-    if feats is None:
-        feats = _ext.row_norm(x.feats, weight, bias, eps, rms=False)
-    return x.replace(feats=feats)
+    return x.replace(feats=_row_norm(x.feats, weight, bias, eps, rms=False))
 
 
 def rms_norm(x: SparseTensor, *, weight=None, eps: float = 1e-5) -> SparseTensor:
@@ -114,10 +111,14 @@ def rms_norm(x: SparseTensor, *, weight=None, eps: float = 1e-5) -> SparseTensor
     ``x.feats`` and ``weight``."""
     if eps <= 0:
         raise ValueError('eps must be positive.')
-    feats = _ext.row_norm_recorded(x.feats, weight, None, eps, rms=True)
-    if feats is None:
-        feats = _ext.row_norm(x.feats, weight, None, eps, rms=True)
-    return x.replace(feats=feats)
+    return x.replace(feats=_row_norm(x.feats, weight, None, eps, rms=True))
+
+
+def _row_norm(feats, weight, bias, eps: float, rms: bool):
+    # only a gradient needs the recorded form, and with it the bindings to torch
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (feats, weight, bias)):
+        return _ext.row_norm_recorded(feats, weight, bias, eps, rms)
+    return _ext.row_norm(feats, weight, bias, eps, rms)
 
 
 def batch_norm(

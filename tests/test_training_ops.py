@@ -7,6 +7,7 @@ import pytest
 import torch
 
 from mlx_lattice_b200 import _ext, _native, nn, ops
+from mlx_lattice_b200.core import SparseTensor
 
 F32, F16 = 0, 1
 
@@ -134,3 +135,25 @@ def test_recurrence_sizes_near_the_end_of_an_int_are_refused():
             _refused(call(64, sequences), 'sequences')
         # the largest ones only lack a workspace
         assert call(top - 1024, top - 64) == _native.LAT_WORKSPACE_TOO_SMALL
+
+
+def test_norms_without_a_gradient_need_no_bindings(monkeypatch):
+    """Inference runs on the C library alone; only a call that records a gradient asks for the
+    extension that is built against torch."""
+    def missing():
+        raise RuntimeError('_bindings.so is not built')
+
+    calls = []
+    monkeypatch.setattr(_ext, 'bindings', missing)
+    monkeypatch.setattr(_ext, 'row_norm', lambda feats, weight, bias, eps, rms: calls.append(rms) or feats)
+    coords = torch.zeros((3, 4), dtype=torch.int32)
+    coords[:, 1] = torch.arange(3)
+    x, weight = SparseTensor(coords, torch.ones((3, 8))), torch.ones(8, requires_grad=True)
+    ops.layer_norm(x)
+    ops.rms_norm(x, weight=weight.detach())
+    with torch.no_grad():
+        ops.layer_norm(x, weight=weight, bias=weight)
+    assert calls == [False, True, False]
+    for call in (ops.layer_norm, ops.rms_norm):
+        with pytest.raises(RuntimeError, match='not built'):
+            call(x, weight=weight)
