@@ -17,6 +17,8 @@ REPO_DIR = os.path.dirname(PACKAGE_DIR)
 CSRC_DIR = os.path.join(PACKAGE_DIR, 'csrc')
 LIBRARY_PATH = os.path.join(PACKAGE_DIR, 'liblattice_b200.so')
 BINDINGS_PATH = os.path.join(PACKAGE_DIR, '_bindings.so')
+# what the bindings were built against: their times say nothing about another torch or Python
+BINDINGS_RECORD = os.path.join(PACKAGE_DIR, '_bindings.built-with')
 BINDINGS_SOURCE = os.path.join(CSRC_DIR, 'bindings.cpp')
 HEADER = os.path.join(REPO_DIR, 'include', 'lattice_b200.h')
 
@@ -61,8 +63,26 @@ def _is_older(target: str, inputs: list[str]) -> bool:
     return any(os.path.getmtime(path) > built for path in inputs)
 
 
+def _bindings_environment() -> str:
+    import torch
+
+    return f'torch {torch.__version__} python {sys.version}'
+
+
+def record_bindings() -> None:
+    with open(BINDINGS_RECORD, 'w') as file:
+        file.write(_bindings_environment())
+
+
+def _bindings_are_stale() -> bool:
+    if _is_older(BINDINGS_PATH, [BINDINGS_SOURCE, HEADER]) or not os.path.exists(BINDINGS_RECORD):
+        return True
+    with open(BINDINGS_RECORD) as file:
+        return file.read() != _bindings_environment()
+
+
 def is_stale() -> bool:
-    return _is_older(LIBRARY_PATH, _inputs()) or _is_older(BINDINGS_PATH, [BINDINGS_SOURCE, HEADER])
+    return _is_older(LIBRARY_PATH, _inputs()) or _bindings_are_stale()
 
 
 def _run(command: list[str], target: str, verbose: bool) -> None:
@@ -107,8 +127,9 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
             *(os.path.join(CSRC_DIR, name) for name in SOURCES),
             '-o', LIBRARY_PATH,
         ], LIBRARY_PATH, verbose)
-    if force or _is_older(BINDINGS_PATH, [BINDINGS_SOURCE, HEADER]):
+    if force or _bindings_are_stale():
         _run(_bindings_command(), BINDINGS_PATH, verbose)
+        record_bindings()
     return LIBRARY_PATH
 
 

@@ -157,3 +157,23 @@ def test_norms_without_a_gradient_need_no_bindings(monkeypatch):
     for call in (ops.layer_norm, ops.rms_norm):
         with pytest.raises(RuntimeError, match='not built'):
             call(x, weight=weight)
+
+
+def test_bindings_count_as_stale_after_a_change_of_torch_or_python(monkeypatch, tmp_path):
+    from mlx_lattice_b200 import build
+
+    for name in ('LIBRARY_PATH', 'BINDINGS_PATH'):
+        path = tmp_path / name
+        path.write_bytes(b'')
+        monkeypatch.setattr(build, name, str(path))
+    monkeypatch.setattr(build, 'BINDINGS_RECORD', str(tmp_path / 'record'))
+    assert build.is_stale()            # nobody knows what they were built against
+    build.record_bindings()
+    assert not build.is_stale()
+    with monkeypatch.context() as change:
+        change.setattr(torch, '__version__', '0.0.1')
+        assert build.is_stale()
+    with monkeypatch.context() as change:
+        change.setattr('sys.version', '3.0')
+        assert build.is_stale()
+    assert not build.is_stale()
