@@ -10,6 +10,7 @@ sequence of calls can be captured into a CUDA graph.
 
 from __future__ import annotations
 
+import warnings
 from typing import Sequence
 
 import torch
@@ -143,10 +144,17 @@ def _second_source(feats: torch.Tensor, feats2) -> tuple[torch.Tensor | None, in
     return feats2, stride2, int(feats2.shape[1])
 
 
+def _say_detached(feats: torch.Tensor) -> None:
+    if feats.requires_grad and torch.is_grad_enabled():
+        warnings.warn('this operator has no gradient: its result is detached from features that require one '
+                      '(layer_norm, rms_norm, dropout and gated_recurrence have gradients).', stacklevel=4)
+
+
 def _feats_arg(feats: torch.Tensor) -> tuple[torch.Tensor, int]:
     _require_cuda(feats, 'feats')
     if feats.ndim != 2:
         raise ValueError('feats must have shape (N, C).')
+    _say_detached(feats)
     if feats.stride(1) != 1:
         feats = feats.contiguous()
     return feats, int(feats.stride(0)) if feats.shape[0] > 1 else int(feats.shape[1])
@@ -633,6 +641,7 @@ def voxelize_features(feats, inverse_rows, voxel_counts, active_rows, reduction)
         raise ValueError('feats must have shape (N, C).')
     if feats.dtype != torch.float32:
         raise ValueError('voxelize currently supports float32 features.')
+    _say_detached(feats)
     if reduction not in ('sum', 'mean'):
         raise ValueError("reduction must be 'sum' or 'mean'.")
     feats = feats.contiguous()
@@ -702,6 +711,7 @@ def interpolate_point_features(voxel_feats, rows, weights):
         raise ValueError('voxel_feats must have shape (N, C).')
     if voxel_feats.dtype != torch.float32:
         raise ValueError('point interpolation currently supports float32.')
+    _say_detached(voxel_feats)
     rows = _i32(rows, 'rows')
     _require_cuda(weights, 'weights')
     if rows.ndim != 2 or rows.shape[1] != 8:

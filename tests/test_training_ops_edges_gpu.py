@@ -427,3 +427,31 @@ def test_recurrence_step_does_not_lose_a_gradient_silently(cuda):
         owner = state.clone().requires_grad_(True)
         _ext.recurrence_step(feats, gate, state, owner)
         assert torch.equal(owner, after)
+
+
+def test_operators_without_a_gradient_say_that_they_detach(cuda):
+    """A projection of this package between two recorded operators cuts the gradient: with a warning,
+    where a gradient is asked for."""
+    import warnings
+
+    from mlx_lattice_b200 import _ext, ops
+
+    feats = torch.ones((8, 16), device=cuda, requires_grad=True)
+    places = torch.zeros((8, 8), dtype=torch.int32, device=cuda)
+    weight = torch.ones((16, 16), device=cuda)
+    x = ops.layer_norm(_sparse(feats))
+    for call in (lambda y: ops.linear(y, weight), ops.silu, ops.relu,
+                 lambda y: ops.batch_norm(y, mean=weight[0], var=weight[0]), lambda y: ops.sparse_add(y, y),
+                 lambda y: _ext.interpolate_point_features(y.feats, places, torch.ones((8, 8), device=cuda))):
+        with pytest.warns(UserWarning, match='no gradient'):
+            call(x)
+        with warnings.catch_warnings():
+            warnings.simplefilter('error')
+            with torch.no_grad():
+                call(x)
+            call(x.replace(feats=x.feats.detach()))
+    with warnings.catch_warnings():   # the recorded ones say nothing
+        warnings.simplefilter('error')
+        ops.rms_norm(x)
+        ops.dropout(x, p=0.5, seed=1)
+        ops.gated_recurrence(x, x, offsets=torch.tensor([0, 8], dtype=torch.int32, device=cuda))
