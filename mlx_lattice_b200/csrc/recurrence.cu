@@ -351,8 +351,8 @@ template <int N> struct Row {
 // Channels c .. c + count - 1 of a thread, at most N, and how they move. Granule: the bytes that
 // move at once, as alignment and channel count allow. Two bytes, float16 rows of an odd width or
 // start: no copy is that small, so the four-byte words that hold the channels move, one more than
-// the channels fill, and are shifted into place when they are read (960,000 x 63: maps 97 us, apply
-// 168, gradient 332; element by element through registers 162, 296, 519).
+// the channels fill, and are shifted into place when they are read (960,000 x 63: maps 104 us, apply
+// 163, gradient 338; element by element through registers 162, 296, 519).
 template <typename T, int N, int Granule> struct Channels {
     static constexpr int kBytes = N * static_cast<int>(sizeof(T));
     static constexpr int kMove = Granule < kBytes ? Granule : kBytes;
@@ -1174,8 +1174,8 @@ int launch_scan(ScanArgs<T> p, void* workspace, size_t bytes, cudaStream_t strea
             return (spans + per_block - 1) / per_block * p.slabs;
         };
         // A walk of two tiles starts less often, a walk of one ends sooner: it is taken where two would
-        // leave multiprocessors idle (2168 x 13 float16 in 94 sequences: 43 us, with two tiles 77;
-        // 15,191 x 12 float32 in 134: 16 against 24).
+        // leave multiprocessors idle (2168 x 13 float16 in 94 sequences: 45 us, with two tiles 77;
+        // 15,191 x 12 float32 in 134: 15 against 24).
         p.span_tiles = blocks_of(2) >= 2 * 148 ? 2 : 1;
         constexpr int kGradientRing = Ring<T, M, Granule, 3, kCarryRows, 2>::kBytes;
         return launch_walk(recurrence_gradient_kernel<T, Granule>, kThreads, kGradientRing,
