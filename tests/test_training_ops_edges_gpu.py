@@ -455,3 +455,41 @@ def test_operators_without_a_gradient_say_that_they_detach(cuda):
         ops.rms_norm(x)
         ops.dropout(x, p=0.5, seed=1)
         ops.gated_recurrence(x, x, offsets=torch.tensor([0, 8], dtype=torch.int32, device=cuda))
+
+
+# --------------------------------------------------------------------------- #
+# norms over frozen features, and their quotient
+# --------------------------------------------------------------------------- #
+
+
+@pytest.mark.parametrize('dtype', DTYPES)
+def test_norm_parameters_alone_over_frozen_features(cuda, dtype):
+    """The first norm over a frozen backbone: features without a gradient, many rows; the bound and
+    its reasons are those of the sums over 200,000 rows beside the other norm tests."""
+    from test_training_ops_gpu import _close, _norm_reference
+
+    from mlx_lattice_b200 import ops
+
+    rng = np.random.default_rng(51)
+    feats, dy = _randn(rng, 200_003, 24, dtype=dtype), _randn(rng, 200_003, 24, dtype=dtype)
+    weight = _randn(rng, 24, dtype=dtype, shift=1.0).requires_grad_(True)
+    bias = _randn(rng, 24, dtype=dtype).requires_grad_(True)
+    y = ops.layer_norm(_sparse(feats), weight=weight, bias=bias).feats
+    dw, db = torch.autograd.grad(y, (weight, bias), dy)
+    want = _norm_reference(_np(feats), _np(weight), _np(bias), _np(dy), 1e-5, False)
+    for got, name in ((y, 'y'), (dw, 'dw'), (db, 'db')):
+        _close(got, *want[name], dtype, name)
+    assert feats.grad is None
+
+
+@pytest.mark.parametrize('channels', [3, 7, 24, 63, 64, 100, 191, 1000, 1023])
+def test_row_means_are_within_one_unit_of_the_quotient(cuda, channels):
+    """Integers whose sums are exact in any order (below 2^24): what is off is the division alone, by at
+    most one unit in the last place, 2^-23 of the mean at most."""
+    from mlx_lattice_b200 import _ext
+
+    rng = np.random.default_rng(channels)
+    x = rng.integers(-8000, 8000, size=(3000, channels)).astype(np.float32)
+    _, mean, _ = _ext.row_norm_forward(torch.from_numpy(x).to(cuda), None, None, 1e-5, False)
+    want = x.astype(np.float64).sum(1) / channels
+    assert (np.abs(_np(mean) - want) <= 2.0 ** -23 * np.abs(want)).all()
